@@ -27,7 +27,8 @@ TENSOR_ARENA = 1
 # kernel ids
 K_EW, K_COPY, K_IM2COL, K_REDUCE, K_GEMM, K_LAYERNORM, K_SOFTMAX, K_ATTN_SCORES, K_GATHER, K_CONV, \
     K_GEMM_TC, K_CONV_TC, K_FLASH_ATTN, K_EMBED, K_STEM_IM2COL, K_GAP_NHWC, K_STEM_CONV, \
-    K_QUANT_E4M3, K_GEMM_FP8, K_QUANT_FP4, K_GEMM_W4A16, K_DEQUANT_FP4, K_WAIT_PROBE, K_GEMM_TF32 = range(1, 25)
+    K_QUANT_E4M3, K_GEMM_FP8, K_QUANT_FP4, K_GEMM_W4A16, K_DEQUANT_FP4, K_WAIT_PROBE, K_GEMM_TF32, \
+    K_ROTARY, K_QK_NORM_ROTARY, K_QK_NORM_APPEND, K_TREE_ATTN, K_KV_COMMIT = range(1, 30)
 KERNEL_NAMES = {
     0: "noop", K_EW: "ew", K_COPY: "copy", K_IM2COL: "im2col", K_REDUCE: "reduce", K_GEMM: "gemm_simt",
     K_LAYERNORM: "layernorm", K_SOFTMAX: "softmax", K_ATTN_SCORES: "attn_scores", K_GATHER: "gather",
@@ -35,6 +36,8 @@ KERNEL_NAMES = {
     K_EMBED: "embed", K_STEM_IM2COL: "stem_im2col", K_GAP_NHWC: "gap_nhwc", K_STEM_CONV: "stem_conv",
     K_QUANT_E4M3: "quant_e4m3", K_GEMM_FP8: "gemm_fp8", K_QUANT_FP4: "quant_fp4", K_GEMM_W4A16: "gemm_w4a16",
     K_DEQUANT_FP4: "dequant_fp4", K_WAIT_PROBE: "wait_probe", K_GEMM_TF32: "gemm_tf32",
+    K_ROTARY: "rotary", K_QK_NORM_ROTARY: "qk_norm_rotary", K_QK_NORM_APPEND: "qk_norm_rotary_append",
+    K_TREE_ATTN: "tree_attention", K_KV_COMMIT: "kv_cache_commit",
 }
 
 # ew ops
@@ -137,6 +140,27 @@ class GapParams(C.Structure):
 
 class WaitProbeParams(C.Structure):
     _fields_ = [("code", C.c_int32)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("scale", C.c_float), ("_pad", C.c_int32)]
+
+
+class QkNormParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("batch", "seq", "capacity")] + \
+               [(n, C.c_int32) for n in ("heads", "kv_heads", "head_dim", "rotary_dim", "interleaved", "normalize",
+                                         "has_q_weight", "has_k_weight")] + \
+               [("epsilon", C.c_float), ("scale", C.c_float)]
+
+
+class TreeAttnParams(C.Structure):
+    _fields_ = [("capacity", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "mask_mode")] + \
+               [("scale", C.c_float), ("_pad", C.c_int32)]
+
+
+class KvCommitParams(C.Structure):
+    _fields_ = [("capacity", C.c_int64)] + [(n, C.c_int32) for n in ("batch", "kv_heads", "head_dim", "path")]
 
 
 EXPORTS = [

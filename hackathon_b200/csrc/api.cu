@@ -86,6 +86,10 @@ static const NameEntry kNames[] = {
     {"b200linearepilogue_bf16", C3B_K_GEMM_TC}, {"b200linearepilogue_fp16", C3B_K_GEMM_TC},
     {"b200flashattention_f32", C3B_K_FLASH_ATTN}, {"b200flashattention_bf16", C3B_K_FLASH_ATTN},
     {"b200flashattention_fp16", C3B_K_FLASH_ATTN},
+    // cached decoding
+    {"rotary_embedding", C3B_K_ROTARY}, {"qk_norm_rotary", C3B_K_QK_NORM_ROTARY},
+    {"qk_norm_rotary_append", C3B_K_QK_NORM_APPEND}, {"tree_attention", C3B_K_TREE_ATTN},
+    {"kv_cache_commit", C3B_K_KV_COMMIT},
 };
 
 static int find_name(const std::string& n) {
@@ -282,6 +286,29 @@ int dispatch(int kid, const c3b_tensor* in, int n_in, const c3b_tensor* out, int
       if ((rc = get_params(params, len, p))) return rc;
       C3B_REQUIRE(n_in >= 1 && n_in <= 3 && n_out == 1, "gap: x [, w [, b]] in, one output");
       return launch_gap_nhwc(in, n_in, out[0], p, s);
+    }
+    case C3B_K_ROTARY: {
+      c3b_rotary_params p;
+      if ((rc = get_params(params, len, p))) return rc;
+      C3B_REQUIRE(n_in == 3 && n_out == 1, "rotary: x, positions, phase steps -> out");
+      return launch_rotary(in, out[0], p, s);
+    }
+    case C3B_K_QK_NORM_ROTARY:
+    case C3B_K_QK_NORM_APPEND: {
+      c3b_qk_norm_params p;
+      if ((rc = get_params(params, len, p))) return rc;
+      return launch_qk_norm_rotary(in, n_in, out, n_out, kid == C3B_K_QK_NORM_APPEND, p, s);
+    }
+    case C3B_K_TREE_ATTN: {
+      c3b_tree_attn_params p;
+      if ((rc = get_params(params, len, p))) return rc;
+      return launch_tree_attn(in, n_in, out, n_out, p, s);
+    }
+    case C3B_K_KV_COMMIT: {
+      c3b_kv_commit_params p;
+      if ((rc = get_params(params, len, p))) return rc;
+      C3B_REQUIRE(n_in == 3 && n_out == 3, "kv commit: lengths, path, accepted -> k cache, v cache, new lengths");
+      return launch_kv_commit(in, out, p, s);
     }
   }
   return fail(C3B_E_UNKNOWN, "unknown kernel id " + std::to_string(kid));

@@ -43,6 +43,15 @@ inline size_t dtype_size(int dt) {
   return 0;
 }
 
+inline bool is_float(int dt) { return dt == C3B_F32 || dt == C3B_BF16 || dt == C3B_F16; }
+
+// Whether two tensors share memory.
+inline bool overlaps(const c3b_tensor& x, const c3b_tensor& y) {
+  const uintptr_t a = (uintptr_t)x.ptr, b = (uintptr_t)y.ptr;
+  const uintptr_t na = numel(x) * dtype_size(x.dtype), nb = numel(y) * dtype_size(y.dtype);
+  return na && nb && a < b + nb && b < a + na;
+}
+
 // Device-side status word: set by kernels whose bounded waits expire.
 extern __device__ int g_status;
 // Limit of one bounded device wait in ns (2 s unless c3b_set_wait_limit_ns
@@ -243,6 +252,13 @@ int launch_dequant_fp4(const c3b_tensor& q, const c3b_tensor& scale, const c3b_t
                        cudaStream_t s);
 int launch_gemm_w4a16(const c3b_tensor* in, int n_in, const c3b_tensor& out, const c3b_gemm_tc_params& p,
                       cudaStream_t s);
+
+int launch_rotary(const c3b_tensor* in, const c3b_tensor& out, const c3b_rotary_params& p, cudaStream_t s);
+int launch_qk_norm_rotary(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, bool append,
+                          const c3b_qk_norm_params& p, cudaStream_t s);
+int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, const c3b_tree_attn_params& p,
+                     cudaStream_t s);
+int launch_kv_commit(const c3b_tensor* in, const c3b_tensor* out, const c3b_kv_commit_params& p, cudaStream_t s);
 
 int sm_count();
 bool launch_stem_tc(const c3b_tensor* in, const c3b_tensor& out, const c3b_stem_conv_params& p, cudaStream_t s,

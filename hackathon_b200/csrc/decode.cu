@@ -1,0 +1,218 @@
+// Attention of drafted tokens over a decoding cache, and the commit of the
+// drafts that were accepted.
+#include <cmath>
+
+#include "common.cuh"
+#include "tc_prims.cuh"
+
+namespace c3b {
+
+namespace dec {
+
+enum { STATUS_ATTN = 41, STATUS_COMMIT = 42 };
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  const int* lengths;
+  const uint8_t* mask;   // null: a chain, each draft sees those before it
+  int64_t mask_stride;   // from one sequence's mask to the next (0: shared)
+  int64_t capacity;
+  int batch, tokens, heads, kv_heads, d, dtype;
+  float scale_log2;
+};
+
+// One block for each query row: four warps stride over the cache rows, each
+// with its own running maximum and sum, joined at the end.
+__global__ void __launch_bounds__(128) tree_rows_kernel(const AttnArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int PL = 8;  // elements a lane: head_dim <= 256
+  __shared__ float part[4][PL * 32], pm[4], pl[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % a.heads;
+  const int64_t token = blockIdx.x / a.heads;
+  const int b = (int)(token / a.tokens), t = (int)(token % a.tokens);
+  const int n = a.lengths[b];
+  const bool fits = n >= 0 && (int64_t)n + a.tokens <= a.capacity;
+  if (!fits && threadIdx.x == 0) atomicExch(&g_status, STATUS_ATTN);
+  const int64_t q0 = (token * a.heads + h) * a.d;
+  const int64_t kv0 = ((int64_t)b * a.kv_heads + h / (a.heads / a.kv_heads)) * a.capacity * a.d;
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride + (int64_t)t * a.tokens : nullptr;
+  float q[PL], o[PL], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    q[i] = lane + 32 * i < a.d ? load_as_f32(a.q, a.dtype, q0 + lane + 32 * i) * a.scale_log2 : 0.f;
+    o[i] = 0.f;
+  }
+  const int end = fits ? n + (mask ? a.tokens : t + 1) : 0;
+  for (int j = warp; j < end; j += 4) {
+    if (j >= n && mask && !mask[j - n]) continue;
+    const int64_t at = kv0 + (int64_t)j * a.d;
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < PL; ++i)
+      if (lane + 32 * i < a.d) x = fmaf(q[i], load_as_f32(a.k, a.dtype, at + lane + 32 * i), x);
+    x = warp_sum(x);
+    const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(m - base), p = exp2f(x - base);
+    m = mn;
+    l = l * f + p;
+#pragma unroll
+    for (int i = 0; i < PL; ++i)
+      if (lane + 32 * i < a.d) o[i] = fmaf(p, load_as_f32(a.v, a.dtype, at + lane + 32 * i), o[i] * f);
+  }
+#pragma unroll
+  for (int i = 0; i < PL; ++i) part[warp][lane + 32 * i] = o[i];
+  if (lane == 0) pm[warp] = m, pl[warp] = l;
+  __syncthreads();
+  float top = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
+  if (top == -INFINITY) top = 0.f;
+  float f[4], sum = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    f[i] = exp2f(pm[i] - top);
+    sum += f[i] * pl[i];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+  for (int i = threadIdx.x; i < a.d; i += 128) {
+    const float x = f[0] * part[0][i] + f[1] * part[1][i] + f[2] * part[2][i] + f[3] * part[3][i];
+    store_from_f32(a.out, a.dtype, q0 + i, x * inv);
+  }
+}
+
+struct CommitArgs {
+  void* cache[2];
+  const int *lengths, *path, *accepted;
+  int* new_lengths;
+  int64_t capacity;
+  int batch, kv_heads, path_len, units;  // units of sizeof(W) bytes a row
+};
+
+// A warp for each sequence, head and cache.  The path rises, so row i never
+// reads what a row before it wrote: a piece is loaded whole, then stored.
+template <typename W>
+__global__ void __launch_bounds__(128) commit_kernel(const CommitArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (item >= (int64_t)a.batch * a.kv_heads * 2) return;
+  const int which = (int)(item & 1);
+  const int64_t bh = item >> 1;
+  const int b = (int)(bh / a.kv_heads);
+  const int n = a.lengths[b], m = a.accepted[b];
+  const int* path = a.path + (int64_t)b * a.path_len;
+  bool ok = n >= 0 && m >= 0 && m <= a.path_len && (int64_t)n + m <= a.capacity;
+  bool moves = false;
+  if (ok) {
+    for (int i = lane; i < m; i += 32) {
+      const int r = path[i], before = i > 0 ? path[i - 1] : -1;
+      ok = ok && r > before && r >= 0 && (int64_t)n + r < a.capacity;
+      moves = moves || r != i;
+    }
+  }
+  ok = __all_sync(0xffffffffu, ok);
+  moves = __any_sync(0xffffffffu, moves);
+  if (lane == 0 && which == 0 && bh % a.kv_heads == 0) {
+    a.new_lengths[b] = ok ? n + m : n;
+    if (!ok) atomicExch(&g_status, STATUS_COMMIT);
+  }
+  if (!ok || !moves) return;
+  W* base = static_cast<W*>(a.cache[which]) + (bh * a.capacity + n) * a.units;
+  constexpr int NB = 4;
+  const int64_t total = (int64_t)m * a.units;
+  for (int64_t e0 = 0; e0 < total; e0 += 32 * NB) {
+    W v[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int64_t e = e0 + 32 * i + lane;
+      if (e < total) v[i] = base[(int64_t)path[e / a.units] * a.units + e % a.units];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int64_t e = e0 + 32 * i + lane;
+      if (e < total) base[e] = v[i];
+    }
+    __syncwarp();
+  }
+}
+
+}  // namespace dec
+
+// in: q, k cache, v cache, lengths, [mask] ; out: o
+int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, const c3b_tree_attn_params& p,
+                     cudaStream_t s) {
+  using namespace dec;
+  C3B_REQUIRE(n_in == (p.mask_mode ? 5 : 4) && n_out == 1, "tree attention: q, k, v, lengths [, mask] -> out");
+  const c3b_tensor &q = in[0], &k = in[1], &v = in[2], &len = in[3];
+  C3B_REQUIRE(is_float(q.dtype) && k.dtype == q.dtype && v.dtype == q.dtype && out[0].dtype == q.dtype,
+              "tree attention: f32, bf16 or fp16, the same for q, caches and output");
+  C3B_REQUIRE(p.batch >= 0 && p.tokens >= 0 && p.heads > 0 && p.kv_heads > 0 && p.heads % p.kv_heads == 0,
+              "tree attention: heads is a multiple of kv_heads");
+  C3B_REQUIRE(p.head_dim >= 1 && p.head_dim <= 256, "tree attention: head_dim is 1 to 256");
+  C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), "tree attention: bad capacity");
+  C3B_REQUIRE(std::isfinite(p.scale), "tree attention: the scale is not finite");
+  const int64_t rows = (int64_t)p.batch * p.tokens * p.heads;
+  C3B_REQUIRE(numel(q) == rows * p.head_dim && numel(out[0]) == numel(q),
+              "tree attention: q and the output are [batch, tokens, heads, head_dim]");
+  const int64_t kv = (int64_t)p.batch * p.kv_heads * p.capacity * p.head_dim;
+  C3B_REQUIRE(numel(k) == kv && numel(v) == kv, "tree attention: caches are [batch, kv_heads, capacity, head_dim]");
+  C3B_REQUIRE(len.dtype == C3B_I32 && numel(len) == p.batch, "tree attention: lengths are int32 [batch]");
+  C3B_REQUIRE(p.mask_mode >= 0 && p.mask_mode <= 2, "tree attention: bad mask mode");
+  const int64_t tt = (int64_t)p.tokens * p.tokens;
+  if (p.mask_mode)
+    C3B_REQUIRE(in[4].dtype == C3B_U8 && numel(in[4]) == (p.mask_mode == 2 ? p.batch * tt : tt),
+                "tree attention: the mask is one byte an entry, [tokens, tokens] or [batch, tokens, tokens]");
+  for (int i = 0; i < n_in; ++i) C3B_REQUIRE(!overlaps(out[0], in[i]), "tree attention: the output overlaps an input");
+  if (rows == 0) return C3B_OK;
+  AttnArgs a = {};
+  a.q = q.ptr, a.k = k.ptr, a.v = v.ptr, a.out = out[0].ptr;
+  a.lengths = (const int*)len.ptr;
+  a.mask = p.mask_mode ? (const uint8_t*)in[4].ptr : nullptr;
+  a.mask_stride = p.mask_mode == 2 ? tt : 0;
+  a.capacity = p.capacity;
+  a.batch = p.batch, a.tokens = p.tokens, a.heads = p.heads, a.kv_heads = p.kv_heads, a.d = p.head_dim;
+  a.dtype = q.dtype;
+  a.scale_log2 = p.scale * 1.4426950408889634f;
+  C3B_REQUIRE(rows < (1ll << 31), "tree attention: too many query rows");
+  return launch_pdl(tree_rows_kernel, (int)rows, 128, 0, s, a);
+}
+
+// in: lengths, path, accepted ; out: k cache, v cache, new lengths
+int launch_kv_commit(const c3b_tensor* in, const c3b_tensor* out, const c3b_kv_commit_params& p, cudaStream_t s) {
+  using namespace dec;
+  const c3b_tensor &len = in[0], &path = in[1], &acc = in[2];
+  C3B_REQUIRE(p.batch >= 0 && p.kv_heads >= 0 && p.head_dim >= 0 && p.path >= 0, "kv commit: bad extents");
+  C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), "kv commit: bad capacity");
+  C3B_REQUIRE(len.dtype == C3B_I32 && numel(len) == p.batch && acc.dtype == C3B_I32 && numel(acc) == p.batch,
+              "kv commit: lengths and accepted are int32 [batch]");
+  C3B_REQUIRE(path.dtype == C3B_I32 && numel(path) == (int64_t)p.batch * p.path, "kv commit: path is int32 [batch, longest path]");
+  const int64_t kv = (int64_t)p.batch * p.kv_heads * p.capacity * p.head_dim;
+  C3B_REQUIRE(is_float(out[0].dtype) && out[1].dtype == out[0].dtype && numel(out[0]) == kv && numel(out[1]) == kv,
+              "kv commit: caches are [batch, kv_heads, capacity, head_dim], of one type");
+  C3B_REQUIRE(out[2].dtype == C3B_I32 && numel(out[2]) == p.batch, "kv commit: the new lengths are int32 [batch]");
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j) {
+      C3B_REQUIRE(!overlaps(out[i], in[j]), "kv commit: an output overlaps an input");
+      C3B_REQUIRE(i == j || !overlaps(out[i], out[j]), "kv commit: the outputs overlap");
+    }
+  if (p.batch == 0) return C3B_OK;
+  C3B_REQUIRE(p.kv_heads > 0, "kv commit: no heads");
+  CommitArgs a = {};
+  a.cache[0] = out[0].ptr, a.cache[1] = out[1].ptr;
+  a.lengths = (const int*)len.ptr, a.path = (const int*)path.ptr, a.accepted = (const int*)acc.ptr;
+  a.new_lengths = (int*)out[2].ptr;
+  a.capacity = p.capacity;
+  a.batch = p.batch, a.kv_heads = p.kv_heads, a.path_len = p.path;
+  const int64_t bytes = (int64_t)p.head_dim * dtype_size(out[0].dtype);
+  const uintptr_t at = (uintptr_t)out[0].ptr | (uintptr_t)out[1].ptr | (uintptr_t)bytes;
+  const int64_t blocks = ((int64_t)p.batch * p.kv_heads * 2 + 3) / 4;
+  C3B_REQUIRE(blocks < (1ll << 31), "kv commit: too many heads");
+  if (at % 16 == 0) {
+    a.units = (int)(bytes / 16);
+    return launch_pdl(commit_kernel<uint4>, (int)blocks, 128, 0, s, a);
+  }
+  a.units = (int)(bytes / 2);
+  return launch_pdl(commit_kernel<uint16_t>, (int)blocks, 128, 0, s, a);
+}
+
+}  // namespace c3b

@@ -1,0 +1,420 @@
+// Rotary positions, per-head query/key RMS norms fused with the rotation, and
+// the append of the rotated keys (and the values) to a decoding cache.
+//
+// One pass over the heads of each token.  With t = position * step_i / 2^64
+// turns, pair i of a head becomes
+//   (a', b') = scale * (a cos 2 pi t - b sin 2 pi t, b cos 2 pi t + a sin 2 pi t),
+// pair i being elements (i, i + R/2) of the head (half layout) or (2i, 2i + 1)
+// (interleaved) of its first R elements; the rest passes through.  Queries and
+// keys are first scaled by w / sqrt(mean(x^2) + eps) where the call normalises.
+//
+// Frequencies come as 64-bit fixed-point fractions of a turn, so the product
+// with an integer position wraps modulo one turn exactly: the range reduction
+// of far positions costs one 64-bit multiplication, loses nothing, and there is
+// no cosine table to read.  The upper 32 bits of the phase go to sincospif.
+//
+// Everything is computed in fp32 and rounded once, to the output's type.
+#include <cmath>
+
+#include "common.cuh"
+#include "tc_prims.cuh"
+
+namespace c3b {
+
+namespace rot {
+
+enum { STATUS_APPEND = 40 };
+
+struct Args {
+  const void* in;       // [tokens, hq + hk + hv, d]
+  void* out[3];         // q, k, v heads: first head of the first token / sequence
+  const float* w[2];    // norm weights of q, k (null: ones)
+  int w_stride[2];      // elements from one head's weights to the next (0: shared)
+  const void* pos;
+  const long long* steps;
+  const int* lengths;   // committed rows of each cache, or null when k and v are written like q
+  int64_t tokens;
+  int64_t capacity;
+  int64_t pos_stride;   // positions from one sequence to the next (0: shared)
+  int seq, heads[3], d, rotary, pos64, interleaved, normalize, copy_v;
+  int64_t out_stride;   // elements from one token to the next in out[0] (and in out[1], out[2] without lengths)
+  int chunks, chunk_heads;
+  float scale, eps;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+
+// N consecutive elements moved as one 4-, 8- or 16-byte word.
+template <int BYTES> struct Word;
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<16> { typedef uint4 type; };
+template <typename T, int N> struct Piece {
+  typedef typename Word<N * sizeof(T)>::type W;
+  union {
+    W w;
+    T v[N];
+  };
+  __device__ __forceinline__ Piece() {}
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const W*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
+};
+
+__device__ __forceinline__ long long position(const Args& a, int64_t b, int64_t t) {
+  const int64_t i = b * a.pos_stride + t;
+  return a.pos64 ? static_cast<const long long*>(a.pos)[i] : (long long)static_cast<const int*>(a.pos)[i];
+}
+
+// scale * (cos, sin) of position * step turns.
+__device__ __forceinline__ void turn(long long pos, long long step, float scale, float& c, float& s) {
+  const unsigned long long phase = (unsigned long long)pos * (unsigned long long)step;
+  const float x = (float)(int)(phase >> 32) * 4.656612873077392578125e-10f;  // 2^-31: half turns in [-1, 1]
+  sincospif(x, &s, &c);
+  c *= scale;
+  s *= scale;
+}
+
+// Where head h of the token goes; null: nowhere.  `role` is 0 (q), 1 (k) or 2 (v).
+template <typename T>
+__device__ __forceinline__ T* destination(const Args& a, int role, int h, int64_t token, int64_t b, int64_t row) {
+  T* base = static_cast<T*>(a.out[role]);
+  if (role == 0 || !a.lengths) return base + token * a.out_stride + (int64_t)h * a.d;
+  if (row < 0) return nullptr;
+  return base + ((b * a.heads[role] + h) * a.capacity + row) * a.d;
+}
+
+// The token's row in the caches; -1 where its sequence does not fit.
+__device__ __forceinline__ int64_t cache_row(const Args& a, int64_t b, int64_t t) {
+  if (!a.lengths) return -1;
+  const int n = a.lengths[b];
+  if (n < 0 || (int64_t)n + a.seq > a.capacity) {
+    atomicExch(&g_status, STATUS_APPEND);
+    return -1;
+  }
+  return n + t;
+}
+
+// A warp takes one token and chunk_heads of its heads; LPH lanes share a head,
+// each with a unit of 2 * VEC elements: VEC pairs, or 2 * VEC elements behind
+// the rotated part.  The sines of a lane's VEC pairs serve all heads of its
+// chunk.  NB heads are loaded before the first is stored.
+template <typename T, int VEC, int LPH, int NB>
+__global__ void __launch_bounds__(256) rotary_kernel(const Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, sub = lane % LPH;
+  constexpr int HPW = 32 / LPH;
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int64_t token = item / a.chunks;
+  if (token >= a.tokens) return;
+  const int64_t b = token / a.seq, t = token - b * a.seq;
+  const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
+  const int first = (int)(item - token * a.chunks) * a.chunk_heads;
+  const int last = min(total, first + a.chunk_heads);
+  const int rotated = a.rotary / (2 * VEC);
+  const bool active = sub < a.d / (2 * VEC), turned = sub < rotated;
+  float c[VEC], s[VEC];
+  if (turned) {
+    const long long pos = position(a, b, t);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) turn(pos, a.steps[sub * VEC + j], a.scale, c[j], s[j]);
+  }
+  // the unit's two pieces: the two halves of its pairs, or two neighbours
+  const bool halves = turned && !a.interleaved;
+  const int off0 = halves ? sub * VEC : sub * 2 * VEC;
+  const int off1 = halves ? a.rotary / 2 + sub * VEC : off0 + VEC;
+  const int64_t row = cache_row(a, b, t);
+  const T* src = static_cast<const T*>(a.in) + token * (int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) * a.d;
+
+  for (int h0 = first; h0 < last; h0 += HPW * NB) {
+    Piece<T, VEC> p0[NB], p1[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int h = h0 + i * HPW + lane / LPH;
+      if (active && h < last) {
+        p0[i].load(src + (int64_t)h * a.d + off0);
+        p1[i].load(src + (int64_t)h * a.d + off1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int h = h0 + i * HPW + lane / LPH;
+      if (h0 + i * HPW >= last) break;  // the same for the whole warp
+      const bool on = active && h < last;
+      const int role = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+      const int hh = h - (role > 0 ? a.heads[0] : 0) - (role > 1 ? a.heads[1] : 0);
+      float x[VEC], y[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        x[j] = on ? to_f32(p0[i].v[j]) : 0.f;
+        y[j] = on ? to_f32(p1[i].v[j]) : 0.f;
+      }
+      if (a.normalize) {
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q = fmaf(x[j], x[j], fmaf(y[j], y[j], q));
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+        if (role < 2 && on) {
+          const float inv = rsqrtf(q / (float)a.d + a.eps);
+          const float* w = a.w[role];
+          if (w) w += (int64_t)hh * a.w_stride[role];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            x[j] *= w ? inv * w[off0 + j] : inv;
+            y[j] *= w ? inv * w[off1 + j] : inv;
+          }
+        }
+      }
+      if (role < 2 && turned) {
+        if (a.interleaved) {
+          // pairs are neighbours: (x0, x1), (x2, x3), ... (y0, y1), ...
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            const float u = x[j], v = x[j + 1];
+            x[j] = u * c[j / 2] - v * s[j / 2];
+            x[j + 1] = v * c[j / 2] + u * s[j / 2];
+            const float m = y[j], n = y[j + 1];
+            y[j] = m * c[(VEC + j) / 2] - n * s[(VEC + j) / 2];
+            y[j + 1] = n * c[(VEC + j) / 2] + m * s[(VEC + j) / 2];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float u = x[j], v = y[j];
+            x[j] = u * c[j] - v * s[j];
+            y[j] = v * c[j] + u * s[j];
+          }
+        }
+      }
+      T* dst = destination<T>(a, role, hh, token, b, row);
+      if (on && dst) {
+        Piece<T, VEC> o0, o1;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          o0.v[j] = from_f32<T>(x[j]);
+          o1.v[j] = from_f32<T>(y[j]);
+        }
+        o0.store(dst + off0);
+        o1.store(dst + off1);
+      }
+    }
+  }
+}
+
+// Any even rotary size, head size and alignment: a warp per head, one pair a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_any_kernel(const Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int64_t token = item / total;
+  if (token >= a.tokens) return;
+  const int h = (int)(item - token * total);
+  const int64_t b = token / a.seq, t = token - b * a.seq;
+  const int role = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+  const int hh = h - (role > 0 ? a.heads[0] : 0) - (role > 1 ? a.heads[1] : 0);
+  const T* src = static_cast<const T*>(a.in) + (token * (a.heads[0] + a.heads[1] + a.heads[2]) + h) * a.d;
+  T* dst = destination<T>(a, role, hh, token, b, cache_row(a, b, t));
+  if (!dst) return;
+  if (role == 2) {
+    for (int i = lane; i < a.d; i += 32) dst[i] = src[i];
+    return;
+  }
+  float inv = 1.f;
+  const float* w = nullptr;
+  if (a.normalize) {
+    float q = 0.f;
+    for (int i = lane; i < a.d; i += 32) {
+      const float x = to_f32(src[i]);
+      q = fmaf(x, x, q);
+    }
+    inv = rsqrtf(warp_sum(q) / (float)a.d + a.eps);
+    if (a.w[role]) w = a.w[role] + (int64_t)hh * a.w_stride[role];
+  }
+  const long long pos = position(a, b, t);
+  for (int p = lane; p < a.rotary / 2; p += 32) {
+    const int i = a.interleaved ? 2 * p : p, j = a.interleaved ? 2 * p + 1 : p + a.rotary / 2;
+    float c, s;
+    turn(pos, a.steps[p], a.scale, c, s);
+    const float u = to_f32(src[i]) * (w ? inv * w[i] : inv), v = to_f32(src[j]) * (w ? inv * w[j] : inv);
+    dst[i] = from_f32<T>(u * c - v * s);
+    dst[j] = from_f32<T>(v * c + u * s);
+  }
+  for (int i = a.rotary + lane; i < a.d; i += 32) dst[i] = from_f32<T>(to_f32(src[i]) * (w ? inv * w[i] : inv));
+}
+
+template <typename T, int VEC, int LPH>
+static int run(Args a, cudaStream_t s) {
+  constexpr int HPW = 32 / LPH, NB = 4;
+  const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
+  const int rounds = (total + HPW - 1) / HPW;
+  // A warp keeps its sines for as many heads as it can; a token's heads are
+  // split over warps only while the tokens alone are fewer than 32 warps an SM.
+  const int64_t want = ((int64_t)sm_count() * 32 + a.tokens - 1) / a.tokens;
+  const int chunks = (int)(want < rounds ? (want < 1 ? 1 : want) : rounds);
+  a.chunk_heads = (rounds + chunks - 1) / chunks * HPW;
+  a.chunks = (total + a.chunk_heads - 1) / a.chunk_heads;
+  const int64_t blocks = (a.tokens * a.chunks + 7) / 8;
+  C3B_REQUIRE(blocks < ((int64_t)1 << 31), "rotary: too many tokens");
+  return launch_pdl(rotary_kernel<T, VEC, LPH, NB>, (int)blocks, 256, 0, s, a);
+}
+
+template <typename T, int VEC>
+static int run_lanes(const Args& a, cudaStream_t s) {
+  const int units = a.d / (2 * VEC);
+  if (units <= 4) return run<T, VEC, 4>(a, s);
+  if (units <= 8) return run<T, VEC, 8>(a, s);
+  if (units <= 16) return run<T, VEC, 16>(a, s);
+  return run<T, VEC, 32>(a, s);
+}
+
+template <typename T>
+static int run_type(const Args& a, cudaStream_t s) {
+  const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
+  if (a.tokens == 0 || total == 0 || a.d == 0) return C3B_OK;
+  // Widest piece (16, 8 or 4 bytes) that divides the rotated part's halves, the
+  // head and every pointer, and leaves at most 32 units a head.
+  uintptr_t at = (uintptr_t)a.in | (uintptr_t)a.out[0] | (uintptr_t)a.out[1] | (uintptr_t)a.out[2];
+  auto fits = [&](int vec) {
+    return a.rotary % (2 * vec) == 0 && a.d % (2 * vec) == 0 && a.d <= 64 * vec && at % (vec * sizeof(T)) == 0;
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (fits(8)) return run_lanes<T, 8>(a, s);
+  }
+  if (fits(4)) return run_lanes<T, 4>(a, s);
+  if (fits(2)) return run_lanes<T, 2>(a, s);
+  const int64_t blocks = (a.tokens * total + 7) / 8;
+  C3B_REQUIRE(blocks < ((int64_t)1 << 31), "rotary: too many heads");
+  return launch_pdl(rotary_any_kernel<T>, (int)blocks, 256, 0, s, a);
+}
+
+static int run_any(const Args& a, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case C3B_F32: return run_type<float>(a, s);
+    case C3B_BF16: return run_type<__nv_bfloat16>(a, s);
+    default: return run_type<__half>(a, s);
+  }
+}
+
+// Positions and phase steps, shared by the three entry points.
+static int take_positions(Args& a, const c3b_tensor& pos, const c3b_tensor& steps, int64_t batch, int64_t seq,
+                          int rotary, const char* who) {
+  const std::string w(who);
+  C3B_REQUIRE(rotary >= 2 && rotary % 2 == 0 && rotary <= a.d, w + ": rotary_dim is even, 2 to head_dim");
+  C3B_REQUIRE(steps.dtype == C3B_I64 && numel(steps) == rotary / 2, w + ": phase steps are int64 [rotary_dim / 2]");
+  C3B_REQUIRE(pos.dtype == C3B_I64 || pos.dtype == C3B_I32, w + ": positions are int64 or int32");
+  const bool shared = pos.ndim == 1 && pos.shape[0] == seq;
+  C3B_REQUIRE(shared || (pos.ndim == 2 && pos.shape[0] == batch && pos.shape[1] == seq),
+              w + ": positions are [batch, tokens] or [tokens]");
+  a.pos = pos.ptr;
+  a.pos64 = pos.dtype == C3B_I64;
+  a.pos_stride = shared ? 0 : seq;
+  a.steps = (const long long*)steps.ptr;
+  a.rotary = rotary;
+  return C3B_OK;
+}
+
+}  // namespace rot
+
+int launch_rotary(const c3b_tensor* in, const c3b_tensor& out, const c3b_rotary_params& p, cudaStream_t s) {
+  using namespace rot;
+  const c3b_tensor &x = in[0], &pos = in[1], &steps = in[2];
+  C3B_REQUIRE(std::isfinite(p.scale), "rotary: the scale is not finite");
+  C3B_REQUIRE(is_float(x.dtype) && out.dtype == x.dtype, "rotary: f32, bf16 or fp16, the same in and out");
+  C3B_REQUIRE(x.ndim == 4, "rotary: x is [batch, tokens, heads, head_dim]");
+  C3B_REQUIRE(numel(out) == numel(x), "rotary: the output is shaped like x");
+  C3B_REQUIRE(x.shape[1] < (1ll << 31) && x.shape[2] < (1 << 24) && x.shape[3] <= 65536, "rotary: extents too large");
+  C3B_REQUIRE(x.ptr == out.ptr || !overlaps(x, out), "rotary: x and the output are the same buffer or do not overlap");
+  Args a = {};
+  a.in = x.ptr;
+  a.out[0] = out.ptr;
+  a.tokens = x.shape[0] * x.shape[1];
+  a.seq = (int)x.shape[1];
+  a.heads[0] = (int)x.shape[2];
+  a.d = (int)x.shape[3];
+  a.out_stride = x.shape[2] * x.shape[3];
+  a.interleaved = p.interleaved != 0;
+  a.scale = p.scale;
+  if (int rc = take_positions(a, pos, steps, x.shape[0], x.shape[1], p.rotary_dim, "rotary")) return rc;
+  return run_any(a, x.dtype, s);
+}
+
+// in: qkv, [q weight], [k weight], positions, phase steps, [lengths when appending]
+int launch_qk_norm_rotary(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, bool append,
+                          const c3b_qk_norm_params& p, cudaStream_t s) {
+  using namespace rot;
+  const char* who = append ? "qk norm rotary append" : "qk norm rotary";
+  const std::string w(who);
+  const int n_w = (p.has_q_weight ? 1 : 0) + (p.has_k_weight ? 1 : 0);
+  C3B_REQUIRE(n_in == 3 + n_w + (append ? 1 : 0) && n_out == (append ? 3 : 1), w + ": wrong number of tensors");
+  const c3b_tensor& x = in[0];
+  const c3b_tensor &pos = in[1 + n_w], &steps = in[2 + n_w];
+  C3B_REQUIRE(p.batch >= 0 && p.seq >= 0 && p.heads >= 0 && p.kv_heads >= 0 && p.head_dim > 0 && p.head_dim <= 65536,
+              w + ": bad extents");
+  C3B_REQUIRE(p.seq < (1ll << 31) && p.heads < (1 << 24) && p.kv_heads < (1 << 24), w + ": extents too large");
+  const int64_t width = p.heads + 2ll * p.kv_heads;
+  C3B_REQUIRE(is_float(x.dtype), w + ": f32, bf16 or fp16");
+  C3B_REQUIRE(numel(x) == p.batch * p.seq * width * p.head_dim, w + ": qkv is [batch, tokens, heads + 2 kv_heads, head_dim]");
+  C3B_REQUIRE(std::isfinite(p.scale) && p.epsilon >= 0.f, w + ": the scale is finite, epsilon at least 0");
+  C3B_REQUIRE(p.normalize || n_w == 0, w + ": weights without normalisation");
+  for (int i = 0; i < n_out; ++i) C3B_REQUIRE(out[i].dtype == x.dtype, w + ": outputs have the type of qkv");
+  Args a = {};
+  a.in = x.ptr;
+  a.tokens = p.batch * p.seq;
+  a.seq = (int)p.seq;
+  a.heads[0] = p.heads;
+  a.heads[1] = a.heads[2] = p.kv_heads;
+  a.d = p.head_dim;
+  a.interleaved = p.interleaved != 0;
+  a.normalize = p.normalize != 0;
+  a.scale = p.scale;
+  a.eps = p.epsilon;
+  int at = 1;
+  for (int role = 0; role < 2; ++role) {
+    if (!(role ? p.has_k_weight : p.has_q_weight)) continue;
+    const c3b_tensor& t = in[at++];
+    const int64_t each = (int64_t)a.heads[role] * a.d;
+    C3B_REQUIRE(t.dtype == C3B_F32 && (numel(t) == a.d || numel(t) == each),
+                w + ": norm weights are f32 [head_dim] or [heads, head_dim]");
+    a.w[role] = (const float*)t.ptr;
+    a.w_stride[role] = numel(t) == a.d ? 0 : a.d;
+  }
+  if (int rc = take_positions(a, pos, steps, p.batch, p.seq, p.rotary_dim, who)) return rc;
+  const size_t es = dtype_size(x.dtype);
+  if (!append) {
+    C3B_REQUIRE(numel(out[0]) == numel(x), w + ": the output is shaped like qkv");
+    C3B_REQUIRE(x.ptr == out[0].ptr || !overlaps(x, out[0]), w + ": qkv and the output are the same buffer or do not overlap");
+    a.out_stride = width * p.head_dim;
+    a.copy_v = x.ptr != out[0].ptr;  // in place, the values already stand where they belong
+    for (int i = 0; i < 3; ++i)
+      a.out[i] = (char*)out[0].ptr + (size_t)(i > 0 ? p.heads : 0) * p.head_dim * es +
+                 (size_t)(i > 1 ? p.kv_heads : 0) * p.head_dim * es;
+    return run_any(a, x.dtype, s);
+  }
+  const c3b_tensor& lengths = in[3 + n_w];
+  C3B_REQUIRE(lengths.dtype == C3B_I32 && numel(lengths) == p.batch, w + ": lengths are int32 [batch]");
+  C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), w + ": bad capacity");
+  C3B_REQUIRE(numel(out[0]) == a.tokens * p.heads * p.head_dim, w + ": the first output is q [batch, tokens, heads, head_dim]");
+  for (int i = 1; i < 3; ++i)
+    C3B_REQUIRE(numel(out[i]) == p.batch * p.kv_heads * p.capacity * p.head_dim,
+                w + ": caches are [batch, kv_heads, capacity, head_dim]");
+  C3B_REQUIRE(!overlaps(out[0], out[1]) && !overlaps(out[0], out[2]) && !overlaps(out[1], out[2]) &&
+                  !overlaps(x, out[0]) && !overlaps(x, out[1]) && !overlaps(x, out[2]),
+              w + ": qkv, q and the caches do not overlap");
+  a.lengths = (const int*)lengths.ptr;
+  a.capacity = p.capacity;
+  a.out_stride = (int64_t)p.heads * p.head_dim;
+  a.copy_v = 1;
+  for (int i = 0; i < 3; ++i) a.out[i] = out[i].ptr;
+  return run_any(a, x.dtype, s);
+}
+
+}  // namespace c3b

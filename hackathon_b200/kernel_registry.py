@@ -30,7 +30,7 @@ from .kernels import Desc, prepare, registered as _prepared_names, resolve as _r
 KernelFunc = Callable[..., None]
 _registry: Dict[str, KernelFunc] = {}
 
-_TYPESTR = {"<f4": L.F32, "<i8": L.I64, "<i4": L.I32, "<f2": L.F16, "|u1": L.U8, "<V2": L.BF16}
+_TYPESTR = {"<f4": L.F32, "<i8": L.I64, "<i4": L.I32, "<f2": L.F16, "|u1": L.U8, "|b1": L.U8, "<V2": L.BF16}
 
 
 def register(name: str) -> Callable[[KernelFunc], KernelFunc]:
@@ -85,7 +85,7 @@ def describe(x: Any) -> Desc:
         if not x.is_contiguous():
             raise ValueError("kernel arrays must be C-contiguous")
         dmap = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16, torch.int64: L.I64,
-                torch.int32: L.I32, torch.uint8: L.U8}
+                torch.int32: L.I32, torch.uint8: L.U8, torch.bool: L.U8}
         return Desc(int(x.data_ptr()), dmap[x.dtype], tuple(int(d) for d in x.shape))
     cai = getattr(x, "__cuda_array_interface__", None)
     if cai is None:

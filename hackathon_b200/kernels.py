@@ -639,6 +639,143 @@ def _b_attn(ins, outs, p):
                     [shape])
 
 
+# ------------------------------------------------------------ cached decoding
+# No reference counterpart: the reference's decoders have learned positions and
+# no cache.  Attribute names follow ONNX's RotaryEmbedding where it has them.
+
+def _exact_out(outs: Sequence[Desc], i: int, shape: Sequence[int], dtype: int, what: str) -> L.Tensor:
+    """An output the kernel updates or fills in its own type: shape and type as they are."""
+    o = outs[i]
+    if o.dtype != dtype or o.numel != int(np.prod(shape, dtype=np.int64)):
+        raise ValueError(f"{what} must be {tuple(shape)} of the inputs' type")
+    return L.make_tensor(o.ptr, dtype, tuple(shape), o.arena)
+
+
+@builder("rotary_embedding")
+def _b_rotary(ins, outs, p):
+    """x [B, S, H, D], positions [B, S] or [S], phase steps [rotary_dim / 2]
+    (hackathon_b200.rotary) -> x rotated; outputs[0] may be x."""
+    if len(ins) != 3 or len(outs) != 1:
+        raise ValueError("rotary_embedding: x, positions, phase steps -> one output")
+    x, pos, steps = ins
+    rp = L.RotaryParams(2 * steps.numel, int(p.get("interleaved", 0)), float(p.get("scale", 1.0)), 0)
+    return Prepared([Launch(L.K_ROTARY, [x.t(), pos.t(), steps.t()], [_exact_out(outs, 0, x.shape, x.dtype, "the output")],
+                            rp)], [x.shape])
+
+
+def _qk_norm_launch(ins, p, name: str, n_in: int) -> Tuple[L.QkNormParams, List[L.Tensor]]:
+    if len(ins) != n_in:
+        raise ValueError(f"{name}: {n_in} inputs (None for an absent weight)")
+    qkv, qw, kw, pos, steps = ins[:5]
+    hq = int(p["num_heads"])
+    hk = int(p.get("kv_num_heads", hq))
+    width = hq + 2 * hk
+    if len(qkv.shape) == 4:
+        if qkv.shape[2] != width:
+            raise ValueError(f"{name}: qkv has {qkv.shape[2]} heads, not num_heads + 2 * kv_num_heads = {width}")
+        d = qkv.shape[3]
+    elif len(qkv.shape) == 3:
+        if not width or qkv.shape[2] % width:
+            raise ValueError(f"{name}: qkv's width {qkv.shape[2]} is not a multiple of {width} heads")
+        d = qkv.shape[2] // width
+    else:
+        raise ValueError(f"{name}: qkv is [B, S, heads, head_dim] or [B, S, heads * head_dim]")
+    q = L.QkNormParams()
+    q.batch, q.seq = qkv.shape[0], qkv.shape[1]
+    q.heads, q.kv_heads, q.head_dim, q.rotary_dim = hq, hk, d, 2 * steps.numel
+    q.interleaved, q.normalize = int(p.get("interleaved", 0)), int(p.get("normalize", 1))
+    q.has_q_weight, q.has_k_weight = int(qw is not None), int(kw is not None)
+    q.epsilon, q.scale = float(p.get("epsilon", 1e-6)), float(p.get("scale", 1.0))
+    tin = [qkv.t()] + [w.t() for w in (qw, kw) if w is not None] + [pos.t(), steps.t()]
+    return q, tin
+
+
+@builder("qk_norm_rotary")
+def _b_qk_norm_rotary(ins, outs, p):
+    """Packed QKV [B, S, Hq + 2 Hkv, D] -> the same with q and k heads RMS-normalised
+    and rotated; outputs[0] may be the input.  With Hkv = Hq the result is what
+    the flash attention kernels read."""
+    q, tin = _qk_norm_launch(ins, p, "qk_norm_rotary", 5)
+    if len(outs) != 1:
+        raise ValueError("qk_norm_rotary: one output")
+    x = ins[0]
+    return Prepared([Launch(L.K_QK_NORM_ROTARY, tin, [_exact_out(outs, 0, x.shape, x.dtype, "the output")], q)],
+                    [x.shape])
+
+
+def _cache_shape(d: Desc, batch: int, name: str) -> Tuple[int, ...]:
+    if len(d.shape) != 4 or d.shape[0] != batch:
+        raise ValueError(f"{name}: caches are [batch, kv_heads, capacity, head_dim]")
+    return d.shape
+
+
+@builder("qk_norm_rotary_append")
+def _b_qk_norm_append(ins, outs, p):
+    """qk_norm_rotary for cached decoding: one more input, lengths int32 [B];
+    outputs q [B, S, Hq, D], k cache and v cache [B, Hkv, capacity, D], whose rows
+    lengths[b] .. lengths[b] + S - 1 are written."""
+    name = "qk_norm_rotary_append"
+    q, tin = _qk_norm_launch(ins, p, name, 6)
+    if len(outs) != 3:
+        raise ValueError(f"{name}: outputs are q, k cache, v cache")
+    x, lengths = ins[0], ins[5]
+    q.capacity = _cache_shape(outs[1], int(q.batch), name)[2]
+    cache = (int(q.batch), int(q.kv_heads), int(q.capacity), int(q.head_dim))
+    if outs[1].shape != cache or outs[2].shape != cache:
+        raise ValueError(f"{name}: caches must be {cache}")
+    shape = (int(q.batch), int(q.seq), int(q.heads), int(q.head_dim))
+    touts = [_exact_out(outs, 0, shape, x.dtype, "q")] + \
+            [_exact_out(outs, i, cache, x.dtype, "a cache") for i in (1, 2)]
+    return Prepared([Launch(L.K_QK_NORM_APPEND, tin + [lengths.t()], touts, q)], [shape, cache, cache])
+
+
+@builder("tree_attention")
+def _b_tree_attention(ins, outs, p):
+    """q [B, T, Hq, D], k cache, v cache [B, Hkv, capacity, D], lengths int32 [B],
+    optional mask (bool or uint8) [T, T] or [B, T, T]: mask[.., i, j] lets draft i
+    see draft j; without one the drafts are a chain.  -> [B, T, Hq, D]."""
+    if len(ins) not in (4, 5) or len(outs) != 1:
+        raise ValueError("tree_attention: q, k cache, v cache, lengths [, mask] -> one output")
+    q, k, v, lengths = ins[:4]
+    mask = ins[4] if len(ins) > 4 else None
+    if len(q.shape) != 4:
+        raise ValueError("tree_attention: q is [batch, tokens, heads, head_dim]")
+    B, T, H, D = q.shape
+    _cache_shape(k, B, "tree_attention")
+    if v.shape != k.shape or k.shape[3] != D:
+        raise ValueError("tree_attention: caches are alike, with q's head_dim")
+    tp = L.TreeAttnParams()
+    tp.capacity = k.shape[2]
+    tp.batch, tp.tokens, tp.heads, tp.kv_heads, tp.head_dim = B, T, H, k.shape[1], D
+    if mask is None:
+        tp.mask_mode = 0
+    elif mask.shape in ((T, T), (B, T, T)):
+        tp.mask_mode = len(mask.shape) - 1
+    else:
+        raise ValueError(f"tree_attention: the mask is [{T}, {T}] or [{B}, {T}, {T}]")
+    scale = p.get("scale")
+    tp.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    tin = [q.t(), k.t(), v.t(), lengths.t()] + ([mask.t()] if mask is not None else [])
+    return Prepared([Launch(L.K_TREE_ATTN, tin, [_exact_out(outs, 0, q.shape, q.dtype, "the output")], tp)], [q.shape])
+
+
+@builder("kv_cache_commit")
+def _b_kv_commit(ins, outs, p):
+    """lengths int32 [B], path int32 [B, A] (accepted drafts, rising), accepted
+    int32 [B]; outputs k cache, v cache (draft path[b, i]'s row moves to row
+    lengths[b] + i, i < accepted[b]) and the new lengths int32 [B]."""
+    if len(ins) != 3 or len(outs) != 3:
+        raise ValueError("kv_cache_commit: lengths, path, accepted -> k cache, v cache, new lengths")
+    lengths, path, acc = ins
+    if len(path.shape) != 2:
+        raise ValueError("kv_cache_commit: path is [batch, longest path]")
+    cache = _cache_shape(outs[0], path.shape[0], "kv_cache_commit")
+    cp = L.KvCommitParams(cache[2], cache[0], cache[1], cache[3], path.shape[1])
+    touts = [_exact_out(outs, i, cache, outs[0].dtype, "a cache") for i in (0, 1)] + \
+            [_exact_out(outs, 2, (cache[0],), L.I32, "the new lengths")]
+    return Prepared([Launch(L.K_KV_COMMIT, [lengths.t(), path.t(), acc.t()], touts, cp)], [cache, cache, (cache[0],)])
+
+
 # ------------------------------------------------------------ data movement
 # kernel_registry.py:669-759, engine.py:1383-1445
 

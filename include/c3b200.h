@@ -92,7 +92,12 @@ enum {
   C3B_K_DEQUANT_FP4 = 22,/* FP4 weights -> bf16 (W4A16 at large M)         */
   C3B_K_WAIT_PROBE = 23, /* failure-path probe: a bounded wait that expires */
   C3B_K_GEMM_TF32 = 24,  /* fp32 x fp32 tcgen05 GEMM as tf32 (kind::tf32) */
-  C3B_K_COUNT = 25
+  C3B_K_ROTARY = 25,     /* rotary positions                              */
+  C3B_K_QK_NORM_ROTARY = 26, /* per-head q/k RMS norm + rotary, packed QKV */
+  C3B_K_QK_NORM_APPEND = 27, /* the same, k and v written into caches      */
+  C3B_K_TREE_ATTN = 28,  /* attention of drafted tokens over a cache      */
+  C3B_K_KV_COMMIT = 29,  /* accepted drafts move together in the caches   */
+  C3B_K_COUNT = 30
 };
 
 /* --- C3B_K_EW: out = program(in0..in5) with NumPy broadcasting.
@@ -308,6 +313,66 @@ typedef struct { int32_t code; } c3b_wait_probe_params;
 typedef struct {
   int64_t n, hw, c;
 } c3b_gap_params;
+
+/* ---------------------------------------------------- cached decoding
+ * No counterpart in the reference, whose decoder Transformers have learned
+ * positions and no cache.  q, k, v and caches share one type (f32, bf16 or
+ * fp16); all arithmetic is fp32, rounded once to the output's type.
+ *
+ * Caches are [batch, kv_heads, capacity, head_dim].  lengths i32 [batch] counts
+ * each sequence's committed rows; the rows of the T tokens of a call follow
+ * them.  lengths is read on the device: a sequence with lengths[b] < 0 or
+ * lengths[b] + T > capacity is left out (nothing appended or committed, its
+ * attention output zero) and sets the device status word (40 append, 41
+ * attention, 42 commit; c3b_device_status, c3b_plan_sync).
+ *
+ * --- C3B_K_ROTARY: inputs x [B, S, H, D], positions i64|i32 [B, S] or [S],
+ * phase steps i64 [rotary_dim / 2]; output shaped like x (x itself: in place).
+ * Pair i of a head's first rotary_dim elements, (i, i + rotary_dim / 2) or
+ * interleaved (2i, 2i + 1), turns by position * step_i / 2^64 turns (wrapping
+ * 64-bit product, so any position is exact) and is multiplied by scale. */
+typedef struct {
+  int32_t rotary_dim, interleaved;
+  float scale;
+  int32_t _pad;
+} c3b_rotary_params;
+
+/* --- C3B_K_QK_NORM_ROTARY: inputs qkv [B, S, heads + 2 kv_heads, D], [q weight],
+ * [k weight] (f32 [D] or [heads, D]; ones when absent), positions, phase steps;
+ * output shaped like qkv (qkv itself: in place): q and k heads
+ * x / sqrt(mean(x^2) + epsilon) * weight (normalize = 1), then rotated, v as is.
+ * --- C3B_K_QK_NORM_APPEND: one more input, lengths; outputs q [B, S, heads, D],
+ * k cache, v cache: token t of sequence b goes to row lengths[b] + t. */
+typedef struct {
+  int64_t batch, seq, capacity; /* capacity: append only */
+  int32_t heads, kv_heads, head_dim, rotary_dim;
+  int32_t interleaved, normalize, has_q_weight, has_k_weight;
+  float epsilon, scale;
+} c3b_qk_norm_params;
+
+/* --- C3B_K_TREE_ATTN: inputs q [B, T, heads, D], k cache, v cache, lengths,
+ * [mask]; output [B, T, heads, D] = softmax(q k^T scale) v.  Draft i of a
+ * sequence sees its committed rows and the drafts j with mask[i][j] != 0 (one
+ * byte each): mask_mode 0 none given, a chain (j <= i); 1 [T, T] for all
+ * sequences; 2 [B, T, T].  A row that sees nothing is zero.  Head h reads kv
+ * head h / (heads / kv_heads).  head_dim 1 to 256.  T = 1 is the decode step. */
+typedef struct {
+  int64_t capacity;
+  int32_t batch, tokens, heads, kv_heads, head_dim, mask_mode;
+  float scale;
+  int32_t _pad;
+} c3b_tree_attn_params;
+
+/* --- C3B_K_KV_COMMIT: inputs lengths, path i32 [B, path] (which drafts were
+ * accepted: rising from 0, in order), accepted i32 [B] (how many of the path
+ * count); outputs k cache, v cache (in place: draft path[i]'s row moves to row
+ * lengths[b] + i), new lengths i32 [B] = lengths + accepted.  A sequence whose
+ * path does not rise or leaves the cache keeps its rows and length and sets the
+ * status word. */
+typedef struct {
+  int64_t capacity;
+  int32_t batch, kv_heads, head_dim, path;
+} c3b_kv_commit_params;
 
 /* ------------------------------------------------------------- entry points */
 
