@@ -165,7 +165,7 @@ class KvCommitParams(C.Structure):
 
 EXPORTS = [
     "c3b_version", "c3b_last_error", "c3b_kernel_id", "c3b_launch", "c3b_device_status", "c3b_sm_count",
-    "c3b_set_wait_limit_ns",
+    "c3b_set_wait_limit_ns", "c3b_tree_attention_workspace",
     "c3b_plan_create", "c3b_plan_destroy", "c3b_plan_arena", "c3b_plan_upload", "c3b_plan_download",
     "c3b_plan_add_input_slot",
     "c3b_plan_add_output_slot", "c3b_plan_slot_ptr", "c3b_plan_add_h2d", "c3b_plan_add_d2h",
@@ -194,6 +194,8 @@ def lib() -> C.CDLL:
     L.c3b_last_error.restype = C.c_char_p
     L.c3b_kernel_id.argtypes = [C.c_char_p]
     L.c3b_launch.argtypes = [i32, T, i32, T, i32, vp, sz, vp]
+    L.c3b_tree_attention_workspace.argtypes = [C.POINTER(TreeAttnParams), i32]
+    L.c3b_tree_attention_workspace.restype = C.c_int64
     L.c3b_device_status.argtypes = [C.POINTER(C.c_int)]
     L.c3b_set_wait_limit_ns.argtypes = [u64]
     L.c3b_plan_create.argtypes = [C.POINTER(vp), u64, i32, i32]
@@ -262,6 +264,20 @@ def launch(kid: int, ins: Sequence[Tensor], outs: Sequence[Tensor], params, stre
     check(L.c3b_launch(kid, ia, len(ins), oa, len(outs), pp, plen, C.c_void_p(stream)), f"{KERNEL_NAMES.get(kid, kid)}")
 
 
+_raw = None
+
+
+def launch_raw():
+    """c3b_launch taking the addresses of its tensor and parameter records."""
+    global _raw
+    if _raw is None:
+        fn = lib()["c3b_launch"]  # a function object of its own, with its own argument types
+        vp, i32 = C.c_void_p, C.c_int
+        fn.argtypes = [i32, vp, i32, vp, i32, vp, C.c_size_t, vp]
+        _raw = fn
+    return _raw
+
+
 def kernel_id(name: str) -> int:
     L = lib()
     rc = L.c3b_kernel_id(name.encode())
@@ -272,6 +288,10 @@ def kernel_id(name: str) -> int:
 
 def set_wait_limit_ns(ns: int) -> None:
     check(lib().c3b_set_wait_limit_ns(int(ns)), "set_wait_limit_ns")
+
+
+def tree_attention_workspace(params: TreeAttnParams, dtype: int) -> int:
+    return check(lib().c3b_tree_attention_workspace(C.byref(params), int(dtype)), "tree_attention_workspace")
 
 
 def device_status() -> int:

@@ -444,6 +444,10 @@ int c3b_launch(int kernel_id, const c3b_tensor* in, int n_in, const c3b_tensor* 
   return dispatch(kernel_id, in, n_in, out, n_out, params, params_len, (cudaStream_t)stream);
 }
 
+int64_t c3b_tree_attention_workspace(const c3b_tree_attn_params* p, int dtype) {
+  return p ? tree_attn_workspace(*p, dtype) : (int64_t)fail(C3B_E_INVALID, "tree attention: no parameters");
+}
+
 int c3b_device_status(int* status) {
   C3B_CHECK_CUDA(cudaDeviceSynchronize());
   int v = 0, zero = 0;

@@ -258,6 +258,7 @@ int launch_qk_norm_rotary(const c3b_tensor* in, int n_in, const c3b_tensor* out,
                           const c3b_qk_norm_params& p, cudaStream_t s);
 int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, const c3b_tree_attn_params& p,
                      cudaStream_t s);
+int64_t tree_attn_workspace(const c3b_tree_attn_params& p, int dtype);
 int launch_kv_commit(const c3b_tensor* in, const c3b_tensor* out, const c3b_kv_commit_params& p, cudaStream_t s);
 
 int sm_count();

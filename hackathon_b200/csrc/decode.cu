@@ -2,29 +2,17 @@
 // drafts that were accepted.
 #include <cmath>
 
-#include "common.cuh"
+#include "decode.cuh"
 #include "tc_prims.cuh"
 
 namespace c3b {
 
 namespace dec {
 
-enum { STATUS_ATTN = 41, STATUS_COMMIT = 42 };
-
-struct AttnArgs {
-  const void *q, *k, *v;
-  void* out;
-  const int* lengths;
-  const uint8_t* mask;   // null: a chain, each draft sees those before it
-  int64_t mask_stride;   // from one sequence's mask to the next (0: shared)
-  int64_t capacity;
-  int batch, tokens, heads, kv_heads, d, dtype;
-  float scale_log2;
-};
-
-// One block for each query row: four warps stride over the cache rows, each
-// with its own running maximum and sum, joined at the end.
-__global__ void __launch_bounds__(128) tree_rows_kernel(const AttnArgs a) {
+// Any type, head size up to 256 and alignment: one block for each query row,
+// four warps stride over the cache rows, each with its own running maximum and
+// sum, joined at the end.
+__global__ void __launch_bounds__(128) tree_rows_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int PL = 8;  // elements a lane: head_dim <= 256
   __shared__ float part[4][PL * 32], pm[4], pl[4];
@@ -77,6 +65,88 @@ __global__ void __launch_bounds__(128) tree_rows_kernel(const AttnArgs a) {
     const float x = f[0] * part[0][i] + f[1] * part[1][i] + f[2] * part[2][i] + f[3] * part[3][i];
     store_from_f32(a.out, a.dtype, q0 + i, x * inv);
   }
+}
+
+// Joins the parts of the segments that were split: a warp for each query row,
+// parts in block order.
+__global__ void __launch_bounds__(256) tree_join_kernel(const Args a, int tile_rows, int64_t items) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (item >= items) return;
+  const int64_t seg = item / tile_rows;
+  const int r = (int)(item - seg * tile_rows);
+  const int64_t bh = seg / a.rtiles;
+  const int row = (int)(seg - bh * a.rtiles) * tile_rows + r;
+  const int2 where = a.segments[seg];
+  if (row >= a.rows || where.x < 0) return;
+  const int first = where.x / 2, parts = where.y - first + 1;
+  auto slot = [&](int i) { return (int64_t)(i ? 2 * (first + i) : where.x) * tile_rows + r; };
+  float mx = -INFINITY;
+  for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, a.part_ml[slot(i)].x);
+  mx = warp_max(mx);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const float2 ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float f = exp2f(ml.x - base);
+    sum += f * ml.y;
+    const int here = min(32, parts - i0);
+#pragma unroll 4
+    for (int i = 0; i < here; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float* p = a.part + slot(i0 + i) * a.d;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = 4 * lane + 128 * k;
+        if (c >= a.d) break;
+        const float4 x = *reinterpret_cast<const float4*>(p + c);
+        o[k].x = fmaf(fi, x.x, o[k].x);
+        o[k].y = fmaf(fi, x.y, o[k].y);
+        o[k].z = fmaf(fi, x.z, o[k].z);
+        o[k].w = fmaf(fi, x.w, o[k].w);
+      }
+    }
+  }
+  sum = warp_sum(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t at = row_offset(a, (int)(bh / a.kv_heads), (int)(bh % a.kv_heads), row);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = 4 * lane + 128 * k;
+    if (c >= a.d) break;
+    const float x[4] = {o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv};
+    for (int j = 0; j < 4; ++j) store_from_f32(a.out, a.dtype, at + c + j, x[j]);
+  }
+}
+
+// Whether the tensor-core kernel takes a call of these sizes: whole 16-byte
+// pieces of a head, cache rows that TMA's 32-bit coordinates reach.
+static bool mma_takes(const c3b_tree_attn_params& p, int dtype) {
+  return dtype != C3B_F32 && p.head_dim % 8 == 0 && p.head_dim <= 256 && p.capacity > 0 &&
+         (int64_t)p.batch * p.kv_heads * p.capacity < (1ll << 31);
+}
+
+static Plan make_plan(const c3b_tree_attn_params& p) {
+  Plan pl = {};
+  const int64_t rows = (int64_t)p.tokens * (p.heads / p.kv_heads);
+  pl.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
+  const int most = pl.dp == 256 ? 32 : 64;
+  pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : most;
+  pl.rtiles = (int)((rows + pl.rows - 1) / pl.rows);
+  pl.segments = (int64_t)p.batch * p.kv_heads * pl.rtiles;
+  const int64_t blocks = (int64_t)sm_count() * mma_blocks_per_sm(pl.dp, pl.rows);
+  const int64_t units = (p.capacity + UNIT - 1) / UNIT;
+  pl.split = units > 4;
+  const int64_t grid = pl.split ? pl.segments * units : pl.segments;
+  pl.grid = (int)(grid < blocks ? grid : blocks);
+  if (pl.split) {
+    pl.part_ml = (size_t)2 * pl.grid * pl.rows * p.head_dim * 4;
+    pl.seg = pl.part_ml + (size_t)2 * pl.grid * pl.rows * 8;
+    pl.bytes = pl.seg + (size_t)pl.segments * 8;
+  }
+  return pl;
 }
 
 struct CommitArgs {
@@ -138,11 +208,17 @@ __global__ void __launch_bounds__(128) commit_kernel(const CommitArgs a) {
 
 }  // namespace dec
 
-// in: q, k cache, v cache, lengths, [mask] ; out: o
+int64_t tree_attn_workspace(const c3b_tree_attn_params& p, int dtype) {
+  if (p.batch <= 0 || p.tokens <= 0 || p.heads <= 0 || p.kv_heads <= 0 || !dec::mma_takes(p, dtype)) return 0;
+  return (int64_t)dec::make_plan(p).bytes;
+}
+
+// in: q, k cache, v cache, lengths, [mask] ; out: o, [workspace]
 int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out, const c3b_tree_attn_params& p,
                      cudaStream_t s) {
   using namespace dec;
-  C3B_REQUIRE(n_in == (p.mask_mode ? 5 : 4) && n_out == 1, "tree attention: q, k, v, lengths [, mask] -> out");
+  C3B_REQUIRE(n_in == (p.mask_mode ? 5 : 4) && (n_out == 1 || n_out == 2),
+              "tree attention: q, k, v, lengths [, mask] -> out [, workspace]");
   const c3b_tensor &q = in[0], &k = in[1], &v = in[2], &len = in[3];
   C3B_REQUIRE(is_float(q.dtype) && k.dtype == q.dtype && v.dtype == q.dtype && out[0].dtype == q.dtype,
               "tree attention: f32, bf16 or fp16, the same for q, caches and output");
@@ -164,16 +240,38 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
                 "tree attention: the mask is one byte an entry, [tokens, tokens] or [batch, tokens, tokens]");
   for (int i = 0; i < n_in; ++i) C3B_REQUIRE(!overlaps(out[0], in[i]), "tree attention: the output overlaps an input");
   if (rows == 0) return C3B_OK;
-  AttnArgs a = {};
+  C3B_REQUIRE(rows < (1ll << 31), "tree attention: too many query rows");
+  Args a = {};
   a.q = q.ptr, a.k = k.ptr, a.v = v.ptr, a.out = out[0].ptr;
   a.lengths = (const int*)len.ptr;
   a.mask = p.mask_mode ? (const uint8_t*)in[4].ptr : nullptr;
   a.mask_stride = p.mask_mode == 2 ? tt : 0;
   a.capacity = p.capacity;
   a.batch = p.batch, a.tokens = p.tokens, a.heads = p.heads, a.kv_heads = p.kv_heads, a.d = p.head_dim;
+  a.group = p.heads / p.kv_heads;
+  a.rows = p.tokens * a.group;
   a.dtype = q.dtype;
   a.scale_log2 = p.scale * 1.4426950408889634f;
-  C3B_REQUIRE(rows < (1ll << 31), "tree attention: too many query rows");
+  const uintptr_t at = (uintptr_t)q.ptr | (uintptr_t)k.ptr | (uintptr_t)v.ptr | (uintptr_t)out[0].ptr;
+  if (mma_takes(p, q.dtype) && at % 16 == 0) {
+    const Plan pl = make_plan(p);
+    if (pl.bytes) {
+      C3B_REQUIRE(n_out == 2 && numel(out[1]) * dtype_size(out[1].dtype) >= pl.bytes && ((uintptr_t)out[1].ptr & 15) == 0,
+                  "tree attention: needs a workspace of " + std::to_string(pl.bytes) + " bytes, 16-byte aligned");
+      for (int i = 0; i < n_in; ++i) C3B_REQUIRE(!overlaps(out[1], in[i]), "tree attention: the workspace overlaps an input");
+      C3B_REQUIRE(!overlaps(out[1], out[0]), "tree attention: the workspace overlaps the output");
+      a.part = (float*)out[1].ptr;
+      a.part_ml = (float2*)((char*)out[1].ptr + pl.part_ml);
+      a.segments = (int2*)((char*)out[1].ptr + pl.seg);
+    }
+    a.rtiles = pl.rtiles;
+    a.split = pl.split;
+    a.min_units = 4;
+    if (int rc = run_mma(q.dtype == C3B_F16, pl, a, s)) return rc;
+    if (!pl.split) return C3B_OK;
+    const int64_t items = pl.segments * pl.rows;
+    return launch_pdl(tree_join_kernel, (int)((items + 7) / 8), 256, 0, s, a, pl.rows, items);
+  }
   return launch_pdl(tree_rows_kernel, (int)rows, 128, 0, s, a);
 }
 

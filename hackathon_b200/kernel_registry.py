@@ -20,12 +20,13 @@ The launch stream is the caller's current stream (CuPy's or torch's), as in
 
 from __future__ import annotations
 
+import ctypes as C
 from typing import Any, Callable, Dict, List, Optional
 
 import numpy as np
 
 from . import _lib as L
-from .kernels import Desc, prepare, registered as _prepared_names, resolve as _resolve_builder
+from .kernels import Desc, prepare, registered as _prepared_names, resolve as _resolve_builder, tree_attention_workspace
 
 KernelFunc = Callable[..., None]
 _registry: Dict[str, KernelFunc] = {}
@@ -192,6 +193,115 @@ def _retype(arr: Any, dt: int) -> Any:
 
 for _name in _prepared_names():
     register(_name)(_make(_name))
+
+
+# ------------------------------------------------------------- cached decoding
+#
+# The decode step calls these once for each layer and token, on buffers whose
+# shapes repeat, so what only depends on shapes, types and attributes (the
+# checks, the parameter block, the tensor records) is kept for them; a call
+# fills in the addresses it was given.  Outputs have their own type and shape.
+
+_WORDS = C.sizeof(L.Tensor) // 8  # a tensor record in 8-byte words, its pointer first
+
+
+class _Ready:
+    __slots__ = ("kid", "n_in", "n_out", "records", "params", "plen", "workspace", "shapes")
+
+
+def _ready(name: str, inputs: List[Any], outputs: List[Any], params: Dict[str, Any]) -> _Ready:
+    ins = [None if x is None else describe(x) for x in inputs]
+    outs = [describe(o) for o in outputs]
+    r = _Ready()
+    r.workspace = 0
+    if name == "tree_attention" and len(outs) == 1 and len(ins) > 1 and \
+            all(d is not None and len(d.shape) == 4 for d in ins[:2]):
+        r.workspace = tree_attention_workspace(ins[0], ins[1])
+        if r.workspace:
+            outs.append(Desc(0, L.U8, (r.workspace,)))
+    prep = prepare(name, ins, outs, params)
+    ln, = prep.launches
+    r.kid, r.n_in, r.n_out, r.params, r.plen = ln.kid, len(ln.ins), len(ln.outs), ln.params, C.sizeof(ln.params)
+    r.records = bytes(L.tensor_array(ln.ins + ln.outs))
+    # outputs given flat come back in their logical shape
+    r.shapes = [(i, s) for i, s in enumerate(prep.out_shapes[:len(outputs)]) if tuple(outputs[i].shape) != tuple(s)]
+    return r
+
+
+def _make_repeated(name: str) -> KernelFunc:
+    generic = _make(name)
+    kept: Dict[Any, _Ready] = {}
+
+    def kernel(inputs: List[Any], outputs: List[Any], params: Dict[str, Any],
+               tuning: Optional[Dict[str, int]] = None) -> None:
+        import torch
+        key: List[Any] = [len(inputs)]
+        ptrs: List[int] = []
+        dev = -1
+        for x in (*inputs, *outputs):
+            if x is None:
+                key.append(None)
+                continue
+            if not isinstance(x, torch.Tensor):
+                return _with_workspace(generic, name, inputs, outputs, params)
+            if not x.is_contiguous():
+                raise ValueError("kernel arrays must be C-contiguous")
+            d = x.get_device()
+            if d != dev:
+                if d < 0:
+                    raise TypeError("kernel arrays must live on the GPU")
+                if dev >= 0:
+                    raise ValueError(f"{name}: arrays on different devices")
+                dev = d
+            key += (x.shape, x.dtype)
+            ptrs.append(x.data_ptr())
+        if dev < 0:
+            raise ValueError(f"{name}: no arrays")
+        if dev != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
+                return kernel(inputs, outputs, params, tuning)
+        key.append(dev)
+        if params:
+            key += params.items()
+        signature = tuple(key)
+        r = kept.get(signature)
+        if r is None:
+            r = _ready(name, inputs, outputs, params or {})
+            if len(kept) >= 512:
+                kept.clear()
+            kept[signature] = r
+        n = r.n_in + r.n_out
+        if r.workspace:
+            scratch = torch.empty(r.workspace, dtype=torch.uint8, device=x.device)
+            ptrs.append(scratch.data_ptr())
+        records = (C.c_uint64 * (n * _WORDS)).from_buffer_copy(r.records)
+        records[0:n * _WORDS:_WORDS] = ptrs
+        at = C.addressof(records)
+        rc = L.launch_raw()(r.kid, at, r.n_in, at + r.n_in * _WORDS * 8, r.n_out, C.addressof(r.params), r.plen,
+                            torch._C._cuda_getCurrentRawStream(dev))
+        if rc < 0:
+            L.check(rc, name)
+        for i, shape in r.shapes:
+            outputs[i] = outputs[i].view(shape)
+
+    kernel.__name__ = f"kernel_{name}"
+    kernel.__qualname__ = kernel.__name__
+    return kernel
+
+
+def _with_workspace(generic: KernelFunc, name: str, inputs: List[Any], outputs: List[Any], params) -> None:
+    """The general path (CuPy and other arrays), with a workspace from the caller's array library."""
+    outs = list(outputs)
+    if name == "tree_attention" and len(outs) == 1:
+        nbytes = tree_attention_workspace(describe(inputs[0]), describe(inputs[1]))
+        if nbytes:
+            outs.append(_scratch(inputs[0], (nbytes,), np.uint8))
+    generic(inputs, outs, params)
+    outputs[:] = outs[:len(outputs)]
+
+
+for _name in ("rotary_embedding", "qk_norm_rotary", "qk_norm_rotary_append", "tree_attention", "kv_cache_commit"):
+    register(_name)(_make_repeated(_name))
 
 
 # ------------------------------------------------------------- fp8 precision path

@@ -733,9 +733,10 @@ def _b_qk_norm_append(ins, outs, p):
 def _b_tree_attention(ins, outs, p):
     """q [B, T, Hq, D], k cache, v cache [B, Hkv, capacity, D], lengths int32 [B],
     optional mask (bool or uint8) [T, T] or [B, T, T]: mask[.., i, j] lets draft i
-    see draft j; without one the drafts are a chain.  -> [B, T, Hq, D]."""
-    if len(ins) not in (4, 5) or len(outs) != 1:
-        raise ValueError("tree_attention: q, k cache, v cache, lengths [, mask] -> one output")
+    see draft j; without one the drafts are a chain.  -> [B, T, Hq, D], and a
+    workspace of at least ``tree_attention_workspace`` bytes where that is not 0."""
+    if len(ins) not in (4, 5) or len(outs) not in (1, 2):
+        raise ValueError("tree_attention: q, k cache, v cache, lengths [, mask] -> output [, workspace]")
     q, k, v, lengths = ins[:4]
     mask = ins[4] if len(ins) > 4 else None
     if len(q.shape) != 4:
@@ -756,7 +757,17 @@ def _b_tree_attention(ins, outs, p):
     scale = p.get("scale")
     tp.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     tin = [q.t(), k.t(), v.t(), lengths.t()] + ([mask.t()] if mask is not None else [])
-    return Prepared([Launch(L.K_TREE_ATTN, tin, [_exact_out(outs, 0, q.shape, q.dtype, "the output")], tp)], [q.shape])
+    touts = [_exact_out(outs, 0, q.shape, q.dtype, "the output")] + [o.t() for o in outs[1:]]
+    return Prepared([Launch(L.K_TREE_ATTN, tin, touts, tp)], [q.shape] + [o.shape for o in outs[1:]])
+
+
+def tree_attention_workspace(q: Desc, k: Desc) -> int:
+    """Bytes of the workspace (its second output) of a tree_attention call."""
+    B, T, H, D = q.shape
+    tp = L.TreeAttnParams()
+    tp.capacity = k.shape[2]
+    tp.batch, tp.tokens, tp.heads, tp.kv_heads, tp.head_dim = B, T, H, k.shape[1], D
+    return L.tree_attention_workspace(tp, q.dtype)
 
 
 @builder("kv_cache_commit")

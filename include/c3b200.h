@@ -355,7 +355,10 @@ typedef struct {
  * sequence sees its committed rows and the drafts j with mask[i][j] != 0 (one
  * byte each): mask_mode 0 none given, a chain (j <= i); 1 [T, T] for all
  * sequences; 2 [B, T, T].  A row that sees nothing is zero.  Head h reads kv
- * head h / (heads / kv_heads).  head_dim 1 to 256.  T = 1 is the decode step. */
+ * head h / (heads / kv_heads).  head_dim 1 to 256.  T = 1 is the decode step.
+ * Second output: a workspace of c3b_tree_attention_workspace bytes, 16-byte
+ * aligned (may be left out where that is 0).  Its contents do not outlast the
+ * call; calls that overlap on the GPU need one each. */
 typedef struct {
   int64_t capacity;
   int32_t batch, tokens, heads, kv_heads, head_dim, mask_mode;
@@ -386,6 +389,9 @@ int c3b_kernel_id(const char* name);
  * Replaces kernel(inputs, outputs, params, tuning) (c35/executor.py:576-581). */
 int c3b_launch(int kernel_id, const c3b_tensor* in, int n_in, const c3b_tensor* out, int n_out,
                const void* params, size_t params_len, void* stream);
+/* Workspace of a C3B_K_TREE_ATTN call on the current device, in bytes; dtype is
+ * that of q and the caches. */
+int64_t c3b_tree_attention_workspace(const c3b_tree_attn_params* p, int dtype);
 /* Read and clear the device-side status word set by kernels whose bounded
  * waits expired (0 = none).  Synchronises the device. */
 int c3b_device_status(int* status);
