@@ -121,24 +121,41 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const Args a, int tile_r
   }
 }
 
-// Whether the tensor-core kernel takes a call of these sizes: whole 16-byte
-// pieces of a head, cache rows that TMA's 32-bit coordinates reach.
-static bool mma_takes(const c3b_tree_attn_params& p, int dtype) {
-  return dtype != C3B_F32 && p.head_dim % 8 == 0 && p.head_dim <= 256 && p.capacity > 0 &&
-         (int64_t)p.batch * p.kv_heads * p.capacity < (1ll << 31);
-}
+// The kernel that takes a call of these sizes: whole 16-byte pieces of a head,
+// and cache rows that TMA's 32-bit coordinates reach; else tree_rows_kernel.
+enum { ROWS_ANY = 0, MMA16, TC16, MMA32 };
 
-static Plan make_plan(const c3b_tree_attn_params& p) {
+static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   Plan pl = {};
+  const bool f32 = dtype == C3B_F32;
+  if (p.head_dim % (f32 ? 4 : 8) || p.head_dim > 256 || p.capacity <= 0 ||
+      (int64_t)p.batch * p.kv_heads * p.capacity >= (1ll << 31))
+    return pl;
   const int64_t rows = (int64_t)p.tokens * (p.heads / p.kv_heads);
   pl.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
-  const int most = pl.dp == 256 ? 32 : 64;
-  pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : most;
+  int unit = 64, per_sm;
+  if (f32) {
+    pl.kernel = MMA32;
+    unit = 32;
+    pl.rows = rows <= 16 || pl.dp == 256 ? 16 : 32;
+    per_sm = f32_blocks_per_sm(pl.dp, pl.rows);
+  } else if (pl.dp <= 128 && rows > 32) {
+    // 33 to 128 rows: one tile for both softmax groups; more: a tile each
+    pl.kernel = TC16;
+    unit = 128;
+    pl.rows = rows <= 128 ? 128 : 256;
+    per_sm = 1;
+  } else {
+    pl.kernel = MMA16;
+    pl.rows = rows <= 16 || pl.dp == 256 ? 16 : 32;
+    per_sm = mma_blocks_per_sm(pl.dp, pl.rows);
+  }
   pl.rtiles = (int)((rows + pl.rows - 1) / pl.rows);
   pl.segments = (int64_t)p.batch * p.kv_heads * pl.rtiles;
-  const int64_t blocks = (int64_t)sm_count() * mma_blocks_per_sm(pl.dp, pl.rows);
-  const int64_t units = (p.capacity + UNIT - 1) / UNIT;
-  pl.split = units > 4;
+  const int64_t blocks = (int64_t)sm_count() * per_sm;
+  const int64_t units = (p.capacity + unit - 1) / unit;
+  pl.split = p.capacity > 256;
+  pl.min_units = 256 / unit;
   const int64_t grid = pl.split ? pl.segments * units : pl.segments;
   pl.grid = (int)(grid < blocks ? grid : blocks);
   if (pl.split) {
@@ -209,8 +226,8 @@ __global__ void __launch_bounds__(128) commit_kernel(const CommitArgs a) {
 }  // namespace dec
 
 int64_t tree_attn_workspace(const c3b_tree_attn_params& p, int dtype) {
-  if (p.batch <= 0 || p.tokens <= 0 || p.heads <= 0 || p.kv_heads <= 0 || !dec::mma_takes(p, dtype)) return 0;
-  return (int64_t)dec::make_plan(p).bytes;
+  if (p.batch <= 0 || p.tokens <= 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads) return 0;
+  return (int64_t)dec::make_plan(p, dtype).bytes;
 }
 
 // in: q, k cache, v cache, lengths, [mask] ; out: o, [workspace]
@@ -226,7 +243,7 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
               "tree attention: heads is a multiple of kv_heads");
   C3B_REQUIRE(p.head_dim >= 1 && p.head_dim <= 256, "tree attention: head_dim is 1 to 256");
   C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), "tree attention: bad capacity");
-  C3B_REQUIRE(std::isfinite(p.scale), "tree attention: the scale is not finite");
+  C3B_REQUIRE(std::isfinite(p.scale) && p.scale > 0.f, "tree attention: the scale is positive");
   const int64_t rows = (int64_t)p.batch * p.tokens * p.heads;
   C3B_REQUIRE(numel(q) == rows * p.head_dim && numel(out[0]) == numel(q),
               "tree attention: q and the output are [batch, tokens, heads, head_dim]");
@@ -253,8 +270,8 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
   a.dtype = q.dtype;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   const uintptr_t at = (uintptr_t)q.ptr | (uintptr_t)k.ptr | (uintptr_t)v.ptr | (uintptr_t)out[0].ptr;
-  if (mma_takes(p, q.dtype) && at % 16 == 0) {
-    const Plan pl = make_plan(p);
+  const Plan pl = make_plan(p, q.dtype);
+  if (pl.kernel != ROWS_ANY && at % 16 == 0) {
     if (pl.bytes) {
       C3B_REQUIRE(n_out == 2 && numel(out[1]) * dtype_size(out[1].dtype) >= pl.bytes && ((uintptr_t)out[1].ptr & 15) == 0,
                   "tree attention: needs a workspace of " + std::to_string(pl.bytes) + " bytes, 16-byte aligned");
@@ -266,8 +283,10 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
     }
     a.rtiles = pl.rtiles;
     a.split = pl.split;
-    a.min_units = 4;
-    if (int rc = run_mma(q.dtype == C3B_F16, pl, a, s)) return rc;
+    a.min_units = pl.min_units;
+    const bool h16 = q.dtype == C3B_F16;
+    if (int rc = pl.kernel == MMA32 ? run_f32(pl, a, s) : pl.kernel == TC16 ? run_tc(h16, pl, a, s) : run_mma(h16, pl, a, s))
+      return rc;
     if (!pl.split) return C3B_OK;
     const int64_t items = pl.segments * pl.rows;
     return launch_pdl(tree_join_kernel, (int)((items + 7) / 8), 256, 0, s, a, pl.rows, items);

@@ -1,6 +1,9 @@
-// What the attention kernels over a decoding cache share (decode.cu, decode_mma.cu):
+// What the attention kernels over a decoding cache share (decode.cu, decode_mma.cu,
+// decode_tc.cu, decode_f32.cu):
 // arguments, the split of the work over blocks, and the walk of a block over its pieces.
 #pragma once
+
+#include <cuda.h>
 
 #include <atomic>
 
@@ -10,8 +13,6 @@ namespace c3b {
 namespace dec {
 
 enum { STATUS_ATTN = 41, STATUS_COMMIT = 42 };
-
-constexpr int UNIT = 64;  // cached rows in a unit of work
 
 struct Args {
   const void *q, *k, *v;
@@ -33,7 +34,8 @@ struct Args {
 
 // How a call runs (host).
 struct Plan {
-  int dp, rows, rtiles, grid, split;
+  int kernel;       // which of them
+  int dp, rows, rtiles, grid, split, min_units;
   int64_t segments;
   size_t part, part_ml, seg, bytes;  // workspace: offsets and size
 };
@@ -52,6 +54,7 @@ struct Walk {
   bool first;       // the block's first piece
 };
 
+template <int UNIT>
 __device__ __forceinline__ void load_sequence(const Args& a, Walk& w) {
   const int n = a.lengths[w.b];
   const bool fits = n >= 0 && (int64_t)n + a.tokens <= a.capacity;
@@ -61,13 +64,16 @@ __device__ __forceinline__ void load_sequence(const Args& a, Walk& w) {
   w.tiles = max(1, (w.end + UNIT - 1) / UNIT);  // one unit at least: somebody writes the zeros
 }
 
+template <int UNIT>
 __device__ __forceinline__ int64_t units_of(const Args& a, int b) {
   const int n = a.lengths[b];
   const bool fits = n >= 0 && (int64_t)n + a.tokens <= a.capacity;
   return (int64_t)max(1, fits ? (n + a.tokens + UNIT - 1) / UNIT : 0) * a.kv_heads * a.rtiles;
 }
 
-// The block's first piece; every warp finds it for itself.
+// The block's first piece, with units of UNIT cached rows; every warp finds it
+// for itself.
+template <int UNIT>
 __device__ __forceinline__ Walk start(const Args& a, int lane) {
   Walk w = {};
   w.first = true;
@@ -80,11 +86,11 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
     if (w.left <= 0) return w;
     w.b = (int)(s0 / per);
     in_b = s0 - (int64_t)w.b * per;
-    load_sequence(a, w);
+    load_sequence<UNIT>(a, w);
     w.count = w.tiles;
   } else {
     int64_t sum = 0;
-    for (int i = lane; i < a.batch; i += 32) sum += units_of(a, i);
+    for (int i = lane; i < a.batch; i += 32) sum += units_of<UNIT>(a, i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     w.total = sum;
@@ -96,7 +102,7 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
     int64_t before = 0;
     for (int i0 = 0;; i0 += 32) {
       // running sums of 32 sequences; the first that reaches past u holds it
-      int64_t x = i0 + lane < a.batch ? units_of(a, i0 + lane) : 0;
+      int64_t x = i0 + lane < a.batch ? units_of<UNIT>(a, i0 + lane) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -112,7 +118,7 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
       }
       before += __shfl_sync(0xffffffffu, x, 31);
     }
-    load_sequence(a, w);
+    load_sequence<UNIT>(a, w);
     in_b = (w.u - before) / w.tiles;
     w.tile = (int)(w.u - before - in_b * w.tiles);
     w.count = (int)min((int64_t)(w.tiles - w.tile), w.left);
@@ -122,6 +128,7 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
   return w;
 }
 
+template <int UNIT>
 __device__ __forceinline__ void next(const Args& a, Walk& w) {
   w.left -= a.split ? w.count : 1;
   if (w.left <= 0) return;
@@ -132,7 +139,7 @@ __device__ __forceinline__ void next(const Args& a, Walk& w) {
     if (++w.head == a.kv_heads) {
       w.head = 0;
       ++w.b;
-      load_sequence(a, w);
+      load_sequence<UNIT>(a, w);
     }
   }
   w.tile = 0;
@@ -179,8 +186,13 @@ inline int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return C3B_OK;
 }
 
+// Tensor maps of the caches: rows of all heads one below the other, boxes of 128 bytes and `box_rows` rows.
+int cache_maps(const Args& a, int box_rows, CUtensorMap* k, CUtensorMap* v);
 int mma_blocks_per_sm(int dp, int rows);
 int run_mma(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
+int run_tc(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
+int f32_blocks_per_sm(int dp, int rows);
+int run_f32(const Plan& pl, const Args& a, cudaStream_t s);
 
 }  // namespace dec
 }  // namespace c3b

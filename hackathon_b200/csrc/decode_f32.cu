@@ -1,0 +1,411 @@
+// fp32 attention of drafted tokens over a decoding cache, on tensor cores.
+//
+// The same operator, split, masks and block layout as decode_mma.cu, with units
+// of 32 cached rows (8 keys a warp).  Products are tf32 (mma.sync m16n8k8) on
+// operands split in two: x = hi + lo, each rounded to tf32's 11 bits, and
+//   x y = hi hi' + hi lo' + lo hi'   (lo lo' is below 2^-22 of the product),
+// each of the three with its own accumulators for the scores, which shortens
+// the chains and adds the small terms to each other first.  A cached row costs
+// 8 D bytes and three times the products, which stays below HBM's time up to 16
+// rows; in plain FMA the same rows would fill the FMA pipe.
+//
+// In P V the k index runs over the keys in the order 0 2 4 6 1 3 5 7: a thread's
+// score accumulators are then its weight operands as they stand, and the eight
+// rows a warp reads of V fall on different banks.
+#include "common.cuh"
+#include "decode.cuh"
+#include "exp2.cuh"
+#include "tc_prims.cuh"
+
+namespace c3b {
+
+namespace df32 {
+using namespace tc;
+using dec::Args;
+
+constexpr int KEYS = 32;
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo, both in tf32.  Where x is not finite hi alone carries it.
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  const float rest = x - __uint_as_float(hi);
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest == rest ? rest : 0.f));
+}
+
+// Byte offset of 16-byte chunk `ch` (4 dims) of row `row` in a tile of 128-byte
+// rows (32 dims) under the 128-byte swizzle; further dims follow in tiles of ROWS rows.
+template <int ROWS>
+__device__ __forceinline__ uint32_t at(int row, int ch) {
+  return (uint32_t)((ch >> 3) * (ROWS * 128) + row * 128 + (((ch ^ row) & 7) << 4));
+}
+
+// DP: head_dim rounded up to 64, 128 or 256.  MT: 16-row tiles.
+template <int DP, int MT>
+struct Shape {
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int CONSUMERS = 4;
+  static constexpr int THREADS = 32 * (CONSUMERS + 1);
+  static constexpr uint32_t TILE = KEYS * DP * 4;
+  static constexpr int OSTRIDE = DP + 8;  // floats: fragment rows fall on different banks
+  static constexpr uint32_t O_BYTES = (uint32_t)ROWS * OSTRIDE * 4;
+  static constexpr uint32_t Q_BYTES = (uint32_t)ROWS * DP * 4;
+  static constexpr uint32_t ML_BYTES = 2u * 4 * ROWS * 4;
+  static constexpr uint32_t QO_BYTES = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;  // the sums are joined where Q stood
+  static constexpr uint32_t REST = QO_BYTES + ML_BYTES + 256;
+  // two blocks an SM where both fit with three stages
+  static constexpr bool PAIR = 3 * 2 * TILE + REST + 1024 <= 113 * 1024;
+  static constexpr uint32_t BUDGET = (PAIR ? 113u : 226u) * 1024;
+  static constexpr int FIT = (int)((BUDGET - REST - 1024) / (2 * TILE));
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static_assert(STAGES >= 2, "a ring needs two stages");
+  static constexpr uint32_t SMEM = STAGES * 2 * TILE + REST + 1024;
+};
+
+template <int DP, int MT>
+__global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR ? 2 : 1))
+    tree_f32_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
+  typedef Shape<DP, MT> S;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_sm = sm + S::STAGES * 2 * S::TILE;
+  float* o_sm = reinterpret_cast<float*>(q_sm);
+  float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [4][ROWS]
+  float* l_sm = m_sm + 4 * S::ROWS;     // [4][ROWS]
+  uint64_t* full = reinterpret_cast<uint64_t*>(l_sm + 4 * S::ROWS);
+  uint64_t* empty = full + S::STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S::STAGES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], S::CONSUMERS);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  dec::Walk w = dec::start<KEYS>(a, lane);
+
+  if (warp == S::CONSUMERS) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (; w.left > 0; dec::next<KEYS>(a, w)) {
+        const int64_t row0 = ((int64_t)w.b * a.kv_heads + w.head) * a.capacity;
+        for (int u = w.tile; u < w.tile + w.count; ++u, ++it) {
+          const uint32_t st = it % S::STAGES;
+          if (!mbar_wait(&empty[st], ((it / S::STAGES) & 1) ^ 1, abort_flag, 43)) goto produced;
+          uint8_t* k_sm = sm + st * 2 * S::TILE;
+          mbar_arrive_tx(&full[st], 2 * S::TILE);
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            tma_load_2d(k_sm + c * (KEYS * 128), &k_map, &full[st], c * 32, (int)(row0 + (int64_t)u * KEYS));
+            tma_load_2d(k_sm + S::TILE + c * (KEYS * 128), &v_map, &full[st], c * 32, (int)(row0 + (int64_t)u * KEYS));
+          }
+        }
+      }
+    produced:;
+    }
+  } else {
+    const int kg = warp;
+    const int g = lane >> 2, t = lane & 3;
+    auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * S::CONSUMERS) : "memory"); };
+    uint32_t it = 0;
+    for (; w.left > 0; dec::next<KEYS>(a, w)) {
+      // ---- the piece's query rows: row r is token r / G, head r % G of the group
+      const int r0 = w.rtile * S::ROWS;
+      const float* q = static_cast<const float*>(a.q);
+      for (int e = threadIdx.x; e < S::ROWS * (DP / 4); e += 32 * S::CONSUMERS) {
+        const int r = e / (DP / 4), ch = e % (DP / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r0 + r < a.rows && ch * 4 < a.d)
+          v = *reinterpret_cast<const float4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 4);
+        *reinterpret_cast<float4*>(q_sm + at<S::ROWS>(r, ch)) = v;
+      }
+      sync();
+      const uint32_t q_base = smem_u32(q_sm);
+      const int qrow = (lane & 7) + ((lane >> 3) & 1) * 8;
+      float o[MT][DP / 8][4], m[MT][2], l[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int nb = 0; nb < DP / 8; ++nb) o[i][nb][0] = o[i][nb][1] = o[i][nb][2] = o[i][nb][3] = 0.f;
+        m[i][0] = m[i][1] = -INFINITY;
+        l[i][0] = l[i][1] = 0.f;
+      }
+
+      for (int u = w.tile; u < w.tile + w.count; ++u, ++it) {
+        const uint32_t st = it % S::STAGES;
+        mbar_wait(&full[st], (it / S::STAGES) & 1, abort_flag, 44);  // on expiry every wait returns: all warps finish
+        uint8_t* v_sm = sm + st * 2 * S::TILE + S::TILE;
+        const uint32_t k_base = smem_u32(sm + st * 2 * S::TILE);
+        // ---- S = Q K^T for the warp's 8 keys: hi hi', hi lo', lo hi'
+        float s[MT][4], acc[MT][3][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int c = 0; c < 3; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
+#pragma unroll 4
+        for (int ks = 0; ks < DP / 8; ks += 2) {
+          uint32_t b[4], bh[4], bl[4];  // two steps of 8 dims
+          ldsm4(k_base + at<KEYS>(kg * 8 + (lane & 7), 2 * ks + (lane >> 3)), b);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) split(__uint_as_float(b[c]), bh[c], bl[c]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t f[4], fh[4], fl[4];
+              ldsm4(q_base + at<S::ROWS>(qrow + 16 * i, 2 * (ks + h) + (lane >> 4)), f);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) split(__uint_as_float(f[c]), fh[c], fl[c]);
+              mma(acc[i][0], fh, bh[2 * h], bh[2 * h + 1]);
+              mma(acc[i][1], fh, bl[2 * h], bl[2 * h + 1]);
+              mma(acc[i][2], fl, bh[2 * h], bh[2 * h + 1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = (acc[i][0][j] + (acc[i][1][j] + acc[i][2][j])) * a.scale_log2;
+        // ---- mask
+        const int key0 = u * KEYS + kg * 8;
+        const bool open = key0 + 8 > w.n;  // the warp's keys reach past the committed rows
+        bool poison = false;
+        if (open) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int r = r0 + 16 * i + 8 * half + g;
+              const int tok = r < a.rows ? r / a.group : 0;
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (!dec::visible(a, w, tok, key0 + 2 * t + j)) s[i][2 * half + j] = -INFINITY;
+            }
+          // rows behind the drafts become zero; drafts are looked at for infinities and NaN
+          for (int e = lane; e < 8 * (DP / 4); e += 32) {
+            const int r = e / (DP / 4), ch = e % (DP / 4);
+            float4* p = reinterpret_cast<float4*>(v_sm + at<KEYS>(kg * 8 + r, ch));
+            if (key0 + r >= w.end) {
+              *p = make_float4(0.f, 0.f, 0.f, 0.f);
+            } else if (key0 + r >= w.n) {
+              const float4 v = *p;
+              const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) poison = poison || !(fabsf(x[k]) < INFINITY);
+            }
+          }
+          fence_proxy_async();  // these writes come before the next load into the stage
+          poison = __any_sync(0xffffffffu, poison);
+        }
+        // ---- running maxima
+        bool grow = false;
+        float top[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x = fmaxf(s[i][2 * half], s[i][2 * half + 1]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            top[i][half] = x;
+            grow = grow || x > m[i][half] + 8.0f;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float mn = fmaxf(m[i][half], top[i][half]);
+              const float f = mn == -INFINITY ? 1.f : exp2f(m[i][half] - mn);
+              m[i][half] = mn;
+              l[i][half] *= f;
+#pragma unroll
+              for (int nb = 0; nb < DP / 8; ++nb) {
+                o[i][nb][2 * half] *= f;
+                o[i][nb][2 * half + 1] *= f;
+              }
+            }
+        }
+        // ---- weights: key 2 t of rows g, g + 8 and key 2 t + 1, as k = t and k = t + 4
+        uint32_t ph[MT][4], pl[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float base = m[i][half] == -INFINITY ? 0.f : m[i][half];
+            float& x = s[i][2 * half];
+            float& y = s[i][2 * half + 1];
+            x = exp2f(x - base);
+            y = exp2f(y - base);
+            l[i][half] += x + y;
+            split(x, ph[i][half], pl[i][half]);
+            split(y, ph[i][2 + half], pl[i][2 + half]);
+          }
+        // ---- O += P V
+        if (!poison) {
+          const int r = kg * 8 + 2 * t;
+#pragma unroll
+          for (int nb = 0; nb < DP / 8; ++nb) {
+            const int ch = 2 * nb + (g >> 2);
+            uint32_t h0, l0, h1, l1;
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r, ch) + 4 * (g & 3)), h0, l0);
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r + 1, ch) + 4 * (g & 3)), h1, l1);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              mma(o[i][nb], pl[i], h0, h1);
+              mma(o[i][nb], ph[i], l0, l1);
+              mma(o[i][nb], ph[i], h0, h1);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int key = 0; key < 8; ++key) {
+            // the key's weights for rows g and g + 8, from the lane that has them
+            float x[MT], y[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              x[i] = __shfl_sync(0xffffffffu, key & 1 ? s[i][1] : s[i][0], (g << 2) | (key >> 1));
+              y[i] = __shfl_sync(0xffffffffu, key & 1 ? s[i][3] : s[i][2], (g << 2) | (key >> 1));
+            }
+#pragma unroll
+            for (int nb = 0; nb < DP / 8; ++nb) {
+              const float2 f = *reinterpret_cast<const float2*>(v_sm + at<KEYS>(kg * 8 + key, 2 * nb + (t >> 1)) + 8 * (t & 1));
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                if (x[i] != 0.f) o[i][nb][0] += x[i] * f.x, o[i][nb][1] += x[i] * f.y;
+                if (y[i] != 0.f) o[i][nb][2] += y[i] * f.x, o[i][nb][3] += y[i] * f.y;
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+      }
+
+      // ---- join the four key groups
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x = l[i][half];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          const int r = 16 * i + 8 * half + g;
+          if (t == 0) m_sm[kg * S::ROWS + r] = m[i][half], l_sm[kg * S::ROWS + r] = x;
+        }
+      sync();
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = 16 * i + 8 * half + g;
+          const float mx = fmaxf(fmaxf(m_sm[r], m_sm[S::ROWS + r]), fmaxf(m_sm[2 * S::ROWS + r], m_sm[3 * S::ROWS + r]));
+          const float f = mx == -INFINITY ? 1.f : exp2f(m[i][half] - mx);
+#pragma unroll
+          for (int nb = 0; nb < DP / 8; ++nb) o[i][nb][2 * half] *= f, o[i][nb][2 * half + 1] *= f;
+        }
+#pragma unroll
+      for (int round = 0; round < 4; ++round) {
+        if (kg == round) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int nb = 0; nb < DP / 8; ++nb) {
+                float2* d = reinterpret_cast<float2*>(o_sm + (16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
+                float2 x = make_float2(o[i][nb][2 * half], o[i][nb][2 * half + 1]);
+                if (round) x.x += d->x, x.y += d->y;
+                *d = x;
+              }
+        }
+        sync();
+      }
+      // ---- out, or to the block's workspace slot
+      const bool whole = w.count == w.tiles;
+      const int slot = dec::slot(w);
+      for (int e = threadIdx.x; e < S::ROWS * (DP / 8); e += 32 * S::CONSUMERS) {
+        const int r = e / (DP / 8), c = e % (DP / 8) * 8;
+        if (r0 + r >= a.rows || c >= a.d) continue;
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, m_sm[i * S::ROWS + r]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sum += mx == -INFINITY ? l_sm[i * S::ROWS + r] : exp2f(m_sm[i * S::ROWS + r] - mx) * l_sm[i * S::ROWS + r];
+        const float* x0 = o_sm + r * S::OSTRIDE + c;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x0[i];
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv;
+          float* dst = static_cast<float*>(a.out) + dec::row_offset(a, w.b, w.head, r0 + r) + c;
+          *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+          if (c + 4 < a.d) *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+          float* dst = a.part + ((int64_t)slot * S::ROWS + r) * a.d + c;
+          *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+          if (c + 4 < a.d) *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          if (c == 0) a.part_ml[(int64_t)slot * S::ROWS + r] = make_float2(mx, sum);
+        }
+      }
+      if (threadIdx.x == 0) dec::note_segment(a, w);
+      sync();
+    }
+  }
+  __syncthreads();
+  if (*abort_flag) {  // loads still in flight land before the block's shared memory is given back
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+}
+
+template <int DP, int MT>
+static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int grid, cudaStream_t s) {
+  typedef Shape<DP, MT> S;
+  auto kernel = tree_f32_kernel<DP, MT>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = dec::allow_smem(kernel, (int)S::SMEM, done)) return rc;
+  return launch_pdl(kernel, grid, S::THREADS, (size_t)S::SMEM, s, km, vm, a);
+}
+
+}  // namespace df32
+
+namespace dec {
+
+int f32_blocks_per_sm(int dp, int rows) {
+  if (dp == 256) return df32::Shape<256, 1>::PAIR ? 2 : 1;
+  if (dp == 128) return (rows == 16 ? df32::Shape<128, 1>::PAIR : df32::Shape<128, 2>::PAIR) ? 2 : 1;
+  return (rows == 16 ? df32::Shape<64, 1>::PAIR : df32::Shape<64, 2>::PAIR) ? 2 : 1;
+}
+
+int run_f32(const Plan& pl, const Args& a, cudaStream_t s) {
+  CUtensorMap km, vm;
+  if (int rc = cache_maps(a, df32::KEYS, &km, &vm)) return rc;
+  if (pl.dp == 64)
+    return pl.rows == 16 ? df32::run<64, 1>(km, vm, a, pl.grid, s) : df32::run<64, 2>(km, vm, a, pl.grid, s);
+  if (pl.dp == 128)
+    return pl.rows == 16 ? df32::run<128, 1>(km, vm, a, pl.grid, s) : df32::run<128, 2>(km, vm, a, pl.grid, s);
+  return df32::run<256, 1>(km, vm, a, pl.grid, s);
+}
+
+}  // namespace dec
+}  // namespace c3b

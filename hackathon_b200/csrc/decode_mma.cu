@@ -17,10 +17,10 @@
 // on timing).  Caches of few units a segment are not cut: block c takes whole
 // segments and nothing is joined.
 //
-// A block: 4 RG consumer warps and one producer.  The producer loads K and V
+// A block: four consumer warps and one producer.  The producer loads K and V
 // units by TMA (128-byte swizzle; dims past head_dim arrive as zeros) into a
-// ring of stages.  Consumer warp (rg, kg) takes 16 MT rows and keys
-// 16 kg .. 16 kg + 15 of every unit, with its own running maximum and sum, so
+// ring of stages.  Consumer warp kg takes all 16 MT rows and keys 16 kg ..
+// 16 kg + 15 of every unit, with its own running maximum and sum, so
 // warps meet only at the end of a piece.  The maximum is raised lazily (by more
 // than 2^8), which skips most rescales of the accumulators.
 //
@@ -39,7 +39,7 @@ namespace dmma {
 using namespace tc;
 using dec::Args;
 
-constexpr int KEYS = dec::UNIT;
+constexpr int KEYS = 64;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -74,20 +74,21 @@ __device__ __forceinline__ uint32_t at(int row, int ch) {
   return (uint32_t)((ch >> 3) * (ROWS * 128) + row * 128 + (((ch ^ row) & 7) << 4));
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  MT: 16-row tiles a warp.  RG: row groups.
-template <int DP, int MT, int RG>
+// DP: head_dim rounded up to 64, 128 or 256.  MT: 16-row tiles.
+template <int DP, int MT>
 struct Shape {
-  static constexpr int ROWS = 16 * MT * RG;
-  static constexpr int CONSUMERS = 4 * RG;
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int CONSUMERS = 4;
   static constexpr int THREADS = 32 * (CONSUMERS + 1);
   static constexpr uint32_t TILE = KEYS * DP * 2;
   static constexpr int OSTRIDE = DP + 8;  // floats: fragment rows fall on different banks
   static constexpr uint32_t O_BYTES = (uint32_t)ROWS * OSTRIDE * 4;
   static constexpr uint32_t Q_BYTES = (uint32_t)ROWS * DP * 2;
   static constexpr uint32_t ML_BYTES = 2u * 4 * ROWS * 4;
-  static constexpr uint32_t REST = O_BYTES + Q_BYTES + ML_BYTES + 256;
-  // two blocks an SM where both fit with three stages (registers allow it for RG = 1)
-  static constexpr bool PAIR = RG == 1 && 3 * 2 * TILE + REST + 1024 <= 113 * 1024;
+  static constexpr uint32_t QO_BYTES = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;  // the sums are joined where Q stood
+  static constexpr uint32_t REST = QO_BYTES + ML_BYTES + 256;
+  // two blocks an SM where both fit with three stages
+  static constexpr bool PAIR = 3 * 2 * TILE + REST + 1024 <= 113 * 1024;
   static constexpr uint32_t BUDGET = (PAIR ? 113u : 226u) * 1024;
   static constexpr int FIT = (int)((BUDGET - REST - 1024) / (2 * TILE));
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
@@ -95,15 +96,15 @@ struct Shape {
   static constexpr uint32_t SMEM = STAGES * 2 * TILE + REST + 1024;
 };
 
-template <int DP, int MT, int RG, bool H16>
-__global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, RG>::PAIR ? 2 : 1))
+template <int DP, int MT, bool H16>
+__global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR ? 2 : 1))
     tree_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
-  typedef Shape<DP, MT, RG> S;
+  typedef Shape<DP, MT> S;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* q_sm = sm + S::STAGES * 2 * S::TILE;
-  float* o_sm = reinterpret_cast<float*>(q_sm + S::Q_BYTES);
-  float* m_sm = o_sm + S::O_BYTES / 4;  // [4][ROWS]
+  float* o_sm = reinterpret_cast<float*>(q_sm);
+  float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [4][ROWS]
   float* l_sm = m_sm + 4 * S::ROWS;     // [4][ROWS]
   uint64_t* full = reinterpret_cast<uint64_t*>(l_sm + 4 * S::ROWS);
   uint64_t* empty = full + S::STAGES;
@@ -121,12 +122,12 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  dec::Walk w = dec::start(a, lane);
+  dec::Walk w = dec::start<KEYS>(a, lane);
 
   if (warp == S::CONSUMERS) {
     if (lane == 0) {
       uint32_t it = 0;
-      for (; w.left > 0; dec::next(a, w)) {
+      for (; w.left > 0; dec::next<KEYS>(a, w)) {
         const int64_t row0 = ((int64_t)w.b * a.kv_heads + w.head) * a.capacity;
         for (int u = w.tile; u < w.tile + w.count; ++u, ++it) {
           const uint32_t st = it % S::STAGES;
@@ -143,11 +144,11 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
     produced:;
     }
   } else {
-    const int rg = warp >> 2, kg = warp & 3;
+    const int kg = warp;
     const int g = lane >> 2, t = lane & 3;
     auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * S::CONSUMERS) : "memory"); };
     uint32_t it = 0;
-    for (; w.left > 0; dec::next(a, w)) {
+    for (; w.left > 0; dec::next<KEYS>(a, w)) {
       // ---- the piece's query rows: row r is token r / G, head r % G of the group
       const int r0 = w.rtile * S::ROWS;
       const uint16_t* q = static_cast<const uint16_t*>(a.q);
@@ -160,8 +161,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
       }
       sync();
       const uint32_t q_base = smem_u32(q_sm);
-      const int wrow = rg * 16 * MT;  // the warp's first row in the tile
-      const int qrow = wrow + (lane & 7) + ((lane >> 3) & 1) * 8;
+      const int qrow = (lane & 7) + ((lane >> 3) & 1) * 8;
       uint32_t qa[MT == 1 ? DP / 16 : 1][4];  // one row tile a warp: its fragments stay in registers
       if constexpr (MT == 1) {
 #pragma unroll
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int r = r0 + wrow + 16 * i + 8 * half + g;
+              const int r = r0 + 16 * i + 8 * half + g;
               const int tok = r < a.rows ? r / a.group : 0;
 #pragma unroll
               for (int nb = 0; nb < 2; ++nb)
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
           float x = l[i][half];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
-          const int r = wrow + 16 * i + 8 * half + g;
+          const int r = 16 * i + 8 * half + g;
           if (t == 0) m_sm[kg * S::ROWS + r] = m[i][half], l_sm[kg * S::ROWS + r] = x;
         }
       sync();
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int r = wrow + 16 * i + 8 * half + g;
+          const int r = 16 * i + 8 * half + g;
           const float mx = fmaxf(fmaxf(m_sm[r], m_sm[S::ROWS + r]), fmaxf(m_sm[2 * S::ROWS + r], m_sm[3 * S::ROWS + r]));
           const float f = mx == -INFINITY ? 1.f : exp2_sfu(m[i][half] - mx);
 #pragma unroll
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
             for (int half = 0; half < 2; ++half)
 #pragma unroll
               for (int nb = 0; nb < DP / 8; ++nb) {
-                float2* d = reinterpret_cast<float2*>(o_sm + (wrow + 16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
+                float2* d = reinterpret_cast<float2*>(o_sm + (16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
                 float2 x = make_float2(o[i][nb][2 * half], o[i][nb][2 * half + 1]);
                 if (round) x.x += d->x, x.y += d->y;
                 *d = x;
@@ -410,10 +410,10 @@ __global__ void __launch_bounds__((Shape<DP, MT, RG>::THREADS), (Shape<DP, MT, R
   }
 }
 
-template <int DP, int MT, int RG, bool H16>
+template <int DP, int MT, bool H16>
 static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int grid, cudaStream_t s) {
-  typedef Shape<DP, MT, RG> S;
-  auto kernel = tree_mma_kernel<DP, MT, RG, H16>;
+  typedef Shape<DP, MT> S;
+  auto kernel = tree_mma_kernel<DP, MT, H16>;
   static std::atomic<uint64_t> done{0};
   if (int rc = dec::allow_smem(kernel, (int)S::SMEM, done)) return rc;
   return launch_pdl(kernel, grid, S::THREADS, (size_t)S::SMEM, s, km, vm, a);
@@ -422,14 +422,10 @@ static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int 
 template <int DP>
 static int run_rows(int rows, bool h16, const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int grid,
                     cudaStream_t s) {
-  if constexpr (DP == 256) {
-    if (rows == 16) return h16 ? run<DP, 1, 1, true>(km, vm, a, grid, s) : run<DP, 1, 1, false>(km, vm, a, grid, s);
-    return h16 ? run<DP, 1, 2, true>(km, vm, a, grid, s) : run<DP, 1, 2, false>(km, vm, a, grid, s);
-  } else {
-    if (rows == 16) return h16 ? run<DP, 1, 1, true>(km, vm, a, grid, s) : run<DP, 1, 1, false>(km, vm, a, grid, s);
-    if (rows == 32) return h16 ? run<DP, 2, 1, true>(km, vm, a, grid, s) : run<DP, 2, 1, false>(km, vm, a, grid, s);
-    return h16 ? run<DP, 2, 2, true>(km, vm, a, grid, s) : run<DP, 2, 2, false>(km, vm, a, grid, s);
+  if constexpr (DP < 256) {
+    if (rows == 32) return h16 ? run<DP, 2, true>(km, vm, a, grid, s) : run<DP, 2, false>(km, vm, a, grid, s);
   }
+  return h16 ? run<DP, 1, true>(km, vm, a, grid, s) : run<DP, 1, false>(km, vm, a, grid, s);
 }
 
 }  // namespace dmma
@@ -438,17 +434,23 @@ namespace dec {
 
 int mma_blocks_per_sm(int dp, int rows) {
   if (dp == 256) return 1;
-  if (dp == 128) return rows == 16 ? dmma::Shape<128, 1, 1>::PAIR + 1 : rows == 32 ? dmma::Shape<128, 2, 1>::PAIR + 1 : 1;
-  return rows == 16 ? dmma::Shape<64, 1, 1>::PAIR + 1 : rows == 32 ? dmma::Shape<64, 2, 1>::PAIR + 1 : 1;
+  if (dp == 128) return (rows == 16 ? dmma::Shape<128, 1>::PAIR : dmma::Shape<128, 2>::PAIR) ? 2 : 1;
+  return (rows == 16 ? dmma::Shape<64, 1>::PAIR : dmma::Shape<64, 2>::PAIR) ? 2 : 1;
+}
+
+int cache_maps(const Args& a, int box_rows, CUtensorMap* k, CUtensorMap* v) {
+  const uint64_t dims[2] = {(uint64_t)a.d, (uint64_t)a.batch * a.kv_heads * a.capacity};
+  const bool f32 = a.dtype == C3B_F32;
+  const uint64_t str[1] = {(uint64_t)a.d * (f32 ? 4 : 2)};
+  const uint32_t box[2] = {f32 ? 32u : 64u, (uint32_t)box_rows};
+  const CUtensorMapDataType dt = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (int rc = encode(k, const_cast<void*>(a.k), 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, dt)) return rc;
+  return encode(v, const_cast<void*>(a.v), 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, dt);
 }
 
 int run_mma(bool h16, const Plan& pl, const Args& a, cudaStream_t s) {
   CUtensorMap km, vm;
-  const uint64_t dims[2] = {(uint64_t)a.d, (uint64_t)a.batch * a.kv_heads * a.capacity};
-  const uint64_t str[1] = {(uint64_t)a.d * 2};
-  const uint32_t box[2] = {64, (uint32_t)UNIT};
-  if (int rc = encode(&km, const_cast<void*>(a.k), 2, dims, str, box)) return rc;
-  if (int rc = encode(&vm, const_cast<void*>(a.v), 2, dims, str, box)) return rc;
+  if (int rc = cache_maps(a, dmma::KEYS, &km, &vm)) return rc;
   switch (pl.dp) {
     case 64: return dmma::run_rows<64>(pl.rows, h16, km, vm, a, pl.grid, s);
     case 128: return dmma::run_rows<128>(pl.rows, h16, km, vm, a, pl.grid, s);

@@ -197,6 +197,7 @@ REFUSED = {
     "tree: output over q": tree_call(q=Desc(1 << 30, L.BF16, (B, S, HQ, D)), out=Desc(1 << 30, L.BF16, (B, S, HQ, D))),
     "tree: output of another type": tree_call(out=lambda n: n(L.F32, B, S, HQ, D)),
     "tree: scale is no number": tree_call({"scale": float("nan")}),
+    "tree: negative scale": tree_call({"scale": -0.125}),
     "commit: path int64": commit_call(path=lambda n: n(L.I64, B, 3)),
     "commit: path rank": commit_call(path=lambda n: n(L.I32, B)),
     "commit: accepted of another size": commit_call(acc=lambda n: n(L.I32, B + 1)),

@@ -251,7 +251,8 @@ TREE = [  # tokens, q heads, kv heads, dim, capacity, lengths
     (5, 4, 4, 64, 300, [0, 7, 123, 290]), (26, 32, 8, 128, 600, [0, 500, 574]), (64, 14, 2, 128, 200, [0, 63, 136]),
     (17, 7, 1, 64, 90, [73, 5]), (33, 24, 3, 64, 1100, [1031, 1067, 0]), (3, 6, 3, 96, 50, [47, 12]), (2, 2, 1, 256, 77, [75]),
     (4, 3, 3, 80, 20, [16, 0]), (2, 4, 2, 17, 30, [28, 3]), (130, 8, 8, 64, 400, [200]), (300, 2, 1, 128, 333, [33, 0]),
-    (1, 64, 1, 128, 5000, [4999]), (9, 128, 1, 64, 257, [240, 248]), (1, 5, 5, 1, 9, [8]),
+    (1, 64, 1, 128, 5000, [4999]), (8, 16, 1, 128, 700, [692, 5]), (16, 16, 2, 128, 1300, [1284, 127, 128, 129]),
+    (7, 40, 1, 64, 2200, [2193, 0]), (11, 12, 1, 96, 900, [889]), (20, 16, 2, 120, 600, [300, 580]), (9, 128, 1, 64, 257, [240, 248]), (1, 5, 5, 1, 9, [8]),
 ]
 
 
@@ -297,10 +298,11 @@ def test_tree_attention(t, case, kind, dtype):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
 @pytest.mark.parametrize("d", [64, 128, 80])
-def test_tree_rows_that_see_nothing_and_masked_poison(t, d, dtype):
+@pytest.mark.parametrize("hq", [2, 4, 12, 32])
+def test_tree_rows_that_see_nothing_and_masked_poison(t, hq, d, dtype):
     """No committed rows and an empty mask row: zero.  Keys and values of drafts that a row does not see are NaN or
     infinite: they do not reach it."""
-    T, hq, hk, cap = 12, 4, 2, 150
+    T, hk, cap = 12, 2, 150
     q, k, v, lengths, _ = tree_inputs(t, (T, hq, hk, d, cap, [0, 0, 130]), dtype)
     mask = np.zeros((3, T, T), bool)
     mask[:, np.arange(T), np.arange(T)] = True
