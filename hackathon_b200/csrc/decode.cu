@@ -68,56 +68,72 @@ __global__ void __launch_bounds__(128) tree_rows_kernel(const Args a) {
 }
 
 // Joins the parts of the segments that were split: a warp for each query row,
-// parts in block order.
-__global__ void __launch_bounds__(256) tree_join_kernel(const Args a, int tile_rows, int64_t items) {
+// parts in block order.  At most 64 registers, so that its blocks fit beside the
+// attention kernel's and are there when that ends.  K: 128-dim halves of a head.
+template <int K>
+__global__ void __launch_bounds__(256, 4) tree_join_kernel(const Args a, int tile_rows, int items) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   if (item >= items) return;
-  const int64_t seg = item / tile_rows;
-  const int r = (int)(item - seg * tile_rows);
-  const int64_t bh = seg / a.rtiles;
-  const int row = (int)(seg - bh * a.rtiles) * tile_rows + r;
+  const int seg = item / tile_rows, r = item - seg * tile_rows;
+  const int bh = seg / a.rtiles, row = (seg - bh * a.rtiles) * tile_rows + r;
+  if (row >= a.rows) return;
   const int2 where = a.segments[seg];
-  if (row >= a.rows || where.x < 0) return;
+  if (where.x < 0) return;
   const int first = where.x / 2, parts = where.y - first + 1;
   auto slot = [&](int i) { return (int64_t)(i ? 2 * (first + i) : where.x) * tile_rows + r; };
-  float mx = -INFINITY;
-  for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, a.part_ml[slot(i)].x);
-  mx = warp_max(mx);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f;
-  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  // 32 parts at a time: their statistics a lane each, then their sums, several on their way together
+  float mx = -INFINITY, sum = 0.f;
+  float4 o[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < parts; i0 += 32) {
     const float2 ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-    const float f = exp2f(ml.x - base);
-    sum += f * ml.y;
+    const float top = fmaxf(mx, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
+    const float f = exp2f(ml.x - base), before = exp2f(mx - base);
+    mx = top;
+    sum = sum * before + f * ml.y;
     const int here = min(32, parts - i0);
-#pragma unroll 4
-    for (int i = 0; i < here; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      const float* p = a.part + slot(i0 + i) * a.d;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int c = 4 * lane + 128 * k;
-        if (c >= a.d) break;
-        const float4 x = *reinterpret_cast<const float4*>(p + c);
-        o[k].x = fmaf(fi, x.x, o[k].x);
-        o[k].y = fmaf(fi, x.y, o[k].y);
-        o[k].z = fmaf(fi, x.z, o[k].z);
-        o[k].w = fmaf(fi, x.w, o[k].w);
+    for (int k = 0; k < K; ++k) {
+      constexpr int NB = 8 / K;
+      o[k].x *= before, o[k].y *= before, o[k].z *= before, o[k].w *= before;
+      const int c = 4 * lane + 128 * k;
+#pragma unroll 1
+      for (int i = 0; i < here; i += NB) {
+        float4 x[NB];
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+          if (c < a.d && i + q < here) x[q] = *reinterpret_cast<const float4*>(a.part + slot(i0 + i + q) * a.d + c);
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+          const float fi = __shfl_sync(0xffffffffu, f, i + q);
+          if (c < a.d && i + q < here) {
+            o[k].x = fmaf(fi, x[q].x, o[k].x);
+            o[k].y = fmaf(fi, x[q].y, o[k].y);
+            o[k].z = fmaf(fi, x[q].z, o[k].z);
+            o[k].w = fmaf(fi, x[q].w, o[k].w);
+          }
+        }
       }
     }
   }
   sum = warp_sum(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t at = row_offset(a, (int)(bh / a.kv_heads), (int)(bh % a.kv_heads), row);
+  const int64_t at = row_offset(a, bh / a.kv_heads, bh % a.kv_heads, row);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < K; ++k) {
     const int c = 4 * lane + 128 * k;
     if (c >= a.d) break;
     const float x[4] = {o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv};
-    for (int j = 0; j < 4; ++j) store_from_f32(a.out, a.dtype, at + c + j, x[j]);
+    if (a.dtype == C3B_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + c) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      const bool h16 = a.dtype == C3B_F16;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at + c) =
+          make_uint2(pack2h(make_float2(x[0], x[1]), h16), pack2h(make_float2(x[2], x[3]), h16));
+    }
   }
 }
 
@@ -157,6 +173,7 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   pl.split = p.capacity > 256;
   pl.min_units = 256 / unit;
   const int64_t grid = pl.split ? pl.segments * units : pl.segments;
+  if (pl.segments * units >= (1ll << 31) || pl.segments * pl.rows >= (1ll << 31)) return Plan{};  // 32-bit counts
   pl.grid = (int)(grid < blocks ? grid : blocks);
   if (pl.split) {
     pl.part_ml = (size_t)2 * pl.grid * pl.rows * p.head_dim * 4;
@@ -288,8 +305,8 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
     if (int rc = pl.kernel == MMA32 ? run_f32(pl, a, s) : pl.kernel == TC16 ? run_tc(h16, pl, a, s) : run_mma(h16, pl, a, s))
       return rc;
     if (!pl.split) return C3B_OK;
-    const int64_t items = pl.segments * pl.rows;
-    return launch_pdl(tree_join_kernel, (int)((items + 7) / 8), 256, 0, s, a, pl.rows, items);
+    const int items = (int)pl.segments * pl.rows;
+    return launch_pdl(p.head_dim <= 128 ? tree_join_kernel<1> : tree_join_kernel<2>, (items + 7) / 8, 256, 0, s, a, pl.rows, items);
   }
   return launch_pdl(tree_rows_kernel, (int)rows, 128, 0, s, a);
 }

@@ -42,33 +42,32 @@ struct Plan {
 
 // A block's way through its pieces.  A segment is one (sequence, kv head, row
 // tile); a piece is the part of a segment that the block has, units tile ..
-// tile + count - 1.
+// tile + count - 1.  All counts fit 32 bits (checked at launch).
 struct Walk {
   int b, head, rtile;
   int n, end;       // committed rows; rows with the drafts (0, 0 where the sequence does not fit)
   int tiles;        // units of the segment
   int tile, count;
-  int64_t left;     // units (split) or segments (not split) still to do, this piece included
-  int64_t u, total; // the piece's first unit among all of them
-  int blocks;       // blocks that have work
+  int left;         // units (split) or segments (not split) still to do, this piece included
+  int u;            // the piece's first unit among all of them
+  int share, extra; // units a block has: share + 1 for the first `extra` blocks, share for the others
   bool first;       // the block's first piece
 };
 
 template <int UNIT>
-__device__ __forceinline__ void load_sequence(const Args& a, Walk& w) {
-  const int n = a.lengths[w.b];
-  const bool fits = n >= 0 && (int64_t)n + a.tokens <= a.capacity;
+__device__ __forceinline__ void set_length(const Args& a, Walk& w, int n) {
+  const bool fits = n >= 0 && n <= (int)a.capacity - a.tokens;
   if (!fits) atomicExch(&g_status, STATUS_ATTN);
   w.n = fits ? n : 0;
   w.end = fits ? n + a.tokens : 0;
   w.tiles = max(1, (w.end + UNIT - 1) / UNIT);  // one unit at least: somebody writes the zeros
 }
 
+// Units of a sequence of n committed rows.
 template <int UNIT>
-__device__ __forceinline__ int64_t units_of(const Args& a, int b) {
-  const int n = a.lengths[b];
-  const bool fits = n >= 0 && (int64_t)n + a.tokens <= a.capacity;
-  return (int64_t)max(1, fits ? (n + a.tokens + UNIT - 1) / UNIT : 0) * a.kv_heads * a.rtiles;
+__device__ __forceinline__ int units_of(const Args& a, int n) {
+  const bool fits = n >= 0 && n <= (int)a.capacity - a.tokens;
+  return max(1, fits ? (n + a.tokens + UNIT - 1) / UNIT : 0) * (a.kv_heads * a.rtiles);
 }
 
 // The block's first piece, with units of UNIT cached rows; every warp finds it
@@ -78,53 +77,56 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
   Walk w = {};
   w.first = true;
   const int per = a.kv_heads * a.rtiles;
-  int64_t in_b;  // the first segment, within its sequence
+  int in_b;  // the first segment, within its sequence
   if (!a.split) {
-    const int64_t segments = (int64_t)a.batch * per;
-    const int64_t s0 = segments * blockIdx.x / gridDim.x;
-    w.left = segments * (blockIdx.x + 1) / gridDim.x - s0;
+    const int segments = a.batch * per;
+    const int share = segments / (int)gridDim.x, extra = segments - share * (int)gridDim.x;
+    const int s0 = (int)blockIdx.x * share + min((int)blockIdx.x, extra);
+    w.left = share + ((int)blockIdx.x < extra);
     if (w.left <= 0) return w;
-    w.b = (int)(s0 / per);
-    in_b = s0 - (int64_t)w.b * per;
-    load_sequence<UNIT>(a, w);
+    w.b = s0 / per;
+    in_b = s0 - w.b * per;
+    set_length<UNIT>(a, w, a.lengths[w.b]);
     w.count = w.tiles;
   } else {
-    int64_t sum = 0;
-    for (int i = lane; i < a.batch; i += 32) sum += units_of<UNIT>(a, i);
+    const int mine = lane < a.batch ? a.lengths[lane] : 0;  // the first 32 sequences stay in registers
+    int sum = lane < a.batch ? units_of<UNIT>(a, mine) : 0;
+    for (int i = 32 + lane; i < a.batch; i += 32) sum += units_of<UNIT>(a, a.lengths[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    w.total = sum;
-    const int64_t most = (sum + a.min_units - 1) / a.min_units;
-    w.blocks = most < gridDim.x ? (int)most : (int)gridDim.x;
-    if ((int)blockIdx.x >= w.blocks) return w;
-    w.u = sum * blockIdx.x / w.blocks;
-    w.left = sum * (blockIdx.x + 1) / w.blocks - w.u;
-    int64_t before = 0;
+    const int blocks = min((int)gridDim.x, (sum + a.min_units - 1) / a.min_units);  // that have work
+    if ((int)blockIdx.x >= blocks) return w;
+    w.share = sum / blocks;
+    w.extra = sum - w.share * blocks;
+    w.u = (int)blockIdx.x * w.share + min((int)blockIdx.x, w.extra);
+    w.left = w.share + ((int)blockIdx.x < w.extra);
+    int before = 0;
     for (int i0 = 0;; i0 += 32) {
       // running sums of 32 sequences; the first that reaches past u holds it
-      int64_t x = i0 + lane < a.batch ? units_of<UNIT>(a, i0 + lane) : 0;
+      const int n = i0 == 0 ? mine : i0 + lane < a.batch ? a.lengths[i0 + lane] : 0;
+      int x = i0 + lane < a.batch ? units_of<UNIT>(a, n) : 0;
+      const int own = x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
       const unsigned past = __ballot_sync(0xffffffffu, before + x > w.u);
       if (past) {
         const int k = __ffs(past) - 1;
-        const int64_t prior = __shfl_sync(0xffffffffu, x, k ? k - 1 : 0);
         w.b = i0 + k;
-        before += k ? prior : 0;
+        before += __shfl_sync(0xffffffffu, x - own, k);
+        set_length<UNIT>(a, w, __shfl_sync(0xffffffffu, n, k));
         break;
       }
       before += __shfl_sync(0xffffffffu, x, 31);
     }
-    load_sequence<UNIT>(a, w);
     in_b = (w.u - before) / w.tiles;
-    w.tile = (int)(w.u - before - in_b * w.tiles);
-    w.count = (int)min((int64_t)(w.tiles - w.tile), w.left);
+    w.tile = w.u - before - in_b * w.tiles;
+    w.count = min(w.tiles - w.tile, w.left);
   }
-  w.head = (int)(in_b / a.rtiles);
-  w.rtile = (int)(in_b - (int64_t)w.head * a.rtiles);
+  w.head = a.rtiles == 1 ? in_b : in_b / a.rtiles;
+  w.rtile = in_b - w.head * a.rtiles;
   return w;
 }
 
@@ -139,11 +141,11 @@ __device__ __forceinline__ void next(const Args& a, Walk& w) {
     if (++w.head == a.kv_heads) {
       w.head = 0;
       ++w.b;
-      load_sequence<UNIT>(a, w);
+      set_length<UNIT>(a, w, a.lengths[w.b]);
     }
   }
   w.tile = 0;
-  w.count = a.split ? (int)min((int64_t)w.tiles, w.left) : w.tiles;
+  w.count = a.split ? min(w.tiles, w.left) : w.tiles;
 }
 
 // The workspace slot of an unfinished piece: a block has one for the segment it
@@ -155,7 +157,9 @@ __device__ __forceinline__ int slot(const Walk& w) { return 2 * blockIdx.x + (w.
 __device__ __forceinline__ void note_segment(const Args& a, const Walk& w) {
   if (!a.split || w.tile != 0) return;
   const int64_t s = ((int64_t)w.b * a.kv_heads + w.head) * a.rtiles + w.rtile;
-  const int last = (int)(((w.u + w.tiles) * w.blocks - 1) / w.total);
+  const int end = w.u + w.tiles - 1;  // the segment's last unit
+  const int large = w.extra * (w.share + 1);
+  const int last = end < large ? end / (w.share + 1) : w.extra + (end - large) / w.share;
   a.segments[s] = w.count == w.tiles ? make_int2(-1, -1) : make_int2(slot(w), last);
 }
 
@@ -165,6 +169,28 @@ __device__ __forceinline__ bool visible(const Args& a, const Walk& w, int tok, i
   if (key >= w.end) return false;
   const int j = key - w.n;
   return a.mask ? a.mask[w.b * a.mask_stride + (int64_t)tok * a.tokens + j] != 0 : j <= tok;
+}
+
+// Which of cache rows key .. key + N - 1 draft `tok` sees, as bits.  The mask's
+// bytes are all in range and none waits for another.
+template <int N>
+__device__ __forceinline__ uint32_t see(const Args& a, const Walk& w, int tok, int key) {
+  const int first = key - w.n;  // the first row among the drafts; below 0: committed
+  const int drafts = w.end - w.n;
+  uint32_t bits = 0;
+  if (first < drafts) {
+    const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_stride + (int64_t)tok * a.tokens : nullptr;
+    uint8_t x[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) x[c] = first + c <= tok;
+    if (mask) {
+#pragma unroll
+      for (int c = 0; c < N; ++c) x[c] = mask[min(max(first + c, 0), a.tokens - 1)];
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) bits |= (uint32_t)(first + c < 0 || (first + c < drafts && x[c] != 0)) << c;
+  }
+  return bits;
 }
 
 // Element offset, in q and the output, of query row r of a kv head.

@@ -12,6 +12,8 @@
 // In P V the k index runs over the keys in the order 0 2 4 6 1 3 5 7: a thread's
 // score accumulators are then its weight operands as they stand, and the eight
 // rows a warp reads of V fall on different banks.
+#include <type_traits>
+
 #include "common.cuh"
 #include "decode.cuh"
 #include "exp2.cuh"
@@ -62,7 +64,7 @@ struct Shape {
   static constexpr int OSTRIDE = DP + 8;  // floats: fragment rows fall on different banks
   static constexpr uint32_t O_BYTES = (uint32_t)ROWS * OSTRIDE * 4;
   static constexpr uint32_t Q_BYTES = (uint32_t)ROWS * DP * 4;
-  static constexpr uint32_t ML_BYTES = 2u * 4 * ROWS * 4;
+  static constexpr uint32_t ML_BYTES = 2u * 5 * ROWS * 4;
   static constexpr uint32_t QO_BYTES = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;  // the sums are joined where Q stood
   static constexpr uint32_t REST = QO_BYTES + ML_BYTES + 256;
   // two blocks an SM where both fit with three stages
@@ -84,7 +86,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
   float* o_sm = reinterpret_cast<float*>(q_sm);
   float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [4][ROWS]
   float* l_sm = m_sm + 4 * S::ROWS;     // [4][ROWS]
-  uint64_t* full = reinterpret_cast<uint64_t*>(l_sm + 4 * S::ROWS);
+  float2* row_sm = reinterpret_cast<float2*>(l_sm + 4 * S::ROWS);  // [ROWS]
+  uint64_t* full = reinterpret_cast<uint64_t*>(row_sm + S::ROWS);
   uint64_t* empty = full + S::STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S::STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -188,15 +191,17 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
         const bool open = key0 + 8 > w.n;  // the warp's keys reach past the committed rows
         bool poison = false;
         if (open) {
+          // a lane looks up a row's 8 keys, all its mask bytes at once
+          const int row = r0 + (lane & (S::ROWS - 1));
+          const uint32_t mine = dec::see<8>(a, w, row < a.rows ? row / a.group : 0, key0);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int r = r0 + 16 * i + 8 * half + g;
-              const int tok = r < a.rows ? r / a.group : 0;
+              const uint32_t bits = __shfl_sync(0xffffffffu, mine, 16 * i + 8 * half + g) >> (2 * t);
 #pragma unroll
               for (int j = 0; j < 2; ++j)
-                if (!dec::visible(a, w, tok, key0 + 2 * t + j)) s[i][2 * half + j] = -INFINITY;
+                if (!(bits >> j & 1)) s[i][2 * half + j] = -INFINITY;
             }
           // rows behind the drafts become zero; drafts are looked at for infinities and NaN
           for (int e = lane; e < 8 * (DP / 4); e += 32) {
@@ -321,41 +326,58 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
           for (int nb = 0; nb < DP / 8; ++nb) o[i][nb][2 * half] *= f, o[i][nb][2 * half + 1] *= f;
         }
+      // In round k warp kg adds a quarter of the dims, quarter (kg + k) mod 4: always the same order, all warps at work.
+      auto add = [&](auto me) {
+        constexpr int KG = decltype(me)::value;
 #pragma unroll
-      for (int round = 0; round < 4; ++round) {
-        if (kg == round) {
+        for (int round = 0; round < 4; ++round) {
+          const int c = (KG + round) & 3;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-              for (int nb = 0; nb < DP / 8; ++nb) {
+              for (int nb = c * (DP / 32); nb < (c + 1) * (DP / 32); ++nb) {
                 float2* d = reinterpret_cast<float2*>(o_sm + (16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
                 float2 x = make_float2(o[i][nb][2 * half], o[i][nb][2 * half + 1]);
-                if (round) x.x += d->x, x.y += d->y;
+                if (round) {
+                  const float2 y = *d;
+                  x.x += y.x, x.y += y.y;
+                }
                 *d = x;
               }
+          if (round == 0 && KG == 0 && lane < S::ROWS) {
+            // the rows' maxima and sums over the four groups
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + lane]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = l_sm[k * S::ROWS + lane];
+              sum += mx == -INFINITY ? x : exp2f(m_sm[k * S::ROWS + lane] - mx) * x;
+            }
+            row_sm[lane] = make_float2(mx, sum);
+          }
+          sync();
         }
-        sync();
-      }
+      };
+      if (kg == 0) add(std::integral_constant<int, 0>());
+      else if (kg == 1) add(std::integral_constant<int, 1>());
+      else if (kg == 2) add(std::integral_constant<int, 2>());
+      else add(std::integral_constant<int, 3>());
       // ---- out, or to the block's workspace slot
       const bool whole = w.count == w.tiles;
       const int slot = dec::slot(w);
       for (int e = threadIdx.x; e < S::ROWS * (DP / 8); e += 32 * S::CONSUMERS) {
         const int r = e / (DP / 8), c = e % (DP / 8) * 8;
         if (r0 + r >= a.rows || c >= a.d) continue;
-        float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, m_sm[i * S::ROWS + r]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sum += mx == -INFINITY ? l_sm[i * S::ROWS + r] : exp2f(m_sm[i * S::ROWS + r] - mx) * l_sm[i * S::ROWS + r];
+        const float2 ml = row_sm[r];
         const float* x0 = o_sm + r * S::OSTRIDE + c;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = x0[i];
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;  // a row that sees nothing is zero
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= inv;
           float* dst = static_cast<float*>(a.out) + dec::row_offset(a, w.b, w.head, r0 + r) + c;
@@ -365,7 +387,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
           float* dst = a.part + ((int64_t)slot * S::ROWS + r) * a.d + c;
           *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
           if (c + 4 < a.d) *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
-          if (c == 0) a.part_ml[(int64_t)slot * S::ROWS + r] = make_float2(mx, sum);
+          if (c == 0) a.part_ml[(int64_t)slot * S::ROWS + r] = ml;
         }
       }
       if (threadIdx.x == 0) dec::note_segment(a, w);

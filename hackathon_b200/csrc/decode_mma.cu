@@ -28,6 +28,8 @@
 // the drafts are zeroed in shared memory (whatever lies there), and a unit
 // whose drafts hold infinities or NaN is multiplied element by element without
 // the masked ones, since 0 times those is not 0.
+#include <type_traits>
+
 #include "common.cuh"
 #include "decode.cuh"
 #include "exp2.cuh"
@@ -84,7 +86,7 @@ struct Shape {
   static constexpr int OSTRIDE = DP + 8;  // floats: fragment rows fall on different banks
   static constexpr uint32_t O_BYTES = (uint32_t)ROWS * OSTRIDE * 4;
   static constexpr uint32_t Q_BYTES = (uint32_t)ROWS * DP * 2;
-  static constexpr uint32_t ML_BYTES = 2u * 4 * ROWS * 4;
+  static constexpr uint32_t ML_BYTES = 2u * 5 * ROWS * 4;
   static constexpr uint32_t QO_BYTES = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;  // the sums are joined where Q stood
   static constexpr uint32_t REST = QO_BYTES + ML_BYTES + 256;
   // two blocks an SM where both fit with three stages
@@ -106,7 +108,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
   float* o_sm = reinterpret_cast<float*>(q_sm);
   float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [4][ROWS]
   float* l_sm = m_sm + 4 * S::ROWS;     // [4][ROWS]
-  uint64_t* full = reinterpret_cast<uint64_t*>(l_sm + 4 * S::ROWS);
+  float2* row_sm = reinterpret_cast<float2*>(l_sm + 4 * S::ROWS);  // [ROWS]
+  uint64_t* full = reinterpret_cast<uint64_t*>(row_sm + S::ROWS);
   uint64_t* empty = full + S::STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S::STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -214,17 +217,19 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[i][nb][j] *= a.scale_log2;
         if (open) {
+          // a lane looks up a row's 16 keys, all its mask bytes at once
+          const int row = r0 + (lane & (S::ROWS - 1));
+          const uint32_t mine = dec::see<16>(a, w, row < a.rows ? row / a.group : 0, key0);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int r = r0 + 16 * i + 8 * half + g;
-              const int tok = r < a.rows ? r / a.group : 0;
+              const uint32_t bits = __shfl_sync(0xffffffffu, mine, 16 * i + 8 * half + g) >> (2 * t);
 #pragma unroll
               for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-                  if (!dec::visible(a, w, tok, key0 + nb * 8 + 2 * t + j)) s[i][nb][2 * half + j] = -INFINITY;
+                  if (!(bits >> (8 * nb + j) & 1)) s[i][nb][2 * half + j] = -INFINITY;
             }
           // rows behind the drafts become zero; drafts are looked at for infinities and NaN
           const uint32_t inf = H16 ? 0x7c00u : 0x7f80u;
@@ -355,41 +360,58 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
           for (int nb = 0; nb < DP / 8; ++nb) o[i][nb][2 * half] *= f, o[i][nb][2 * half + 1] *= f;
         }
+      // In round k warp kg adds a quarter of the dims, quarter (kg + k) mod 4: always the same order, all warps at work.
+      auto add = [&](auto me) {
+        constexpr int KG = decltype(me)::value;
 #pragma unroll
-      for (int round = 0; round < 4; ++round) {
-        if (kg == round) {
+        for (int round = 0; round < 4; ++round) {
+          const int c = (KG + round) & 3;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-              for (int nb = 0; nb < DP / 8; ++nb) {
+              for (int nb = c * (DP / 32); nb < (c + 1) * (DP / 32); ++nb) {
                 float2* d = reinterpret_cast<float2*>(o_sm + (16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
                 float2 x = make_float2(o[i][nb][2 * half], o[i][nb][2 * half + 1]);
-                if (round) x.x += d->x, x.y += d->y;
+                if (round) {
+                  const float2 y = *d;
+                  x.x += y.x, x.y += y.y;
+                }
                 *d = x;
               }
+          if (round == 0 && KG == 0 && lane < S::ROWS) {
+            // the rows' maxima and sums over the four groups
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + lane]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = l_sm[k * S::ROWS + lane];
+              sum += mx == -INFINITY ? x : exp2_sfu(m_sm[k * S::ROWS + lane] - mx) * x;
+            }
+            row_sm[lane] = make_float2(mx, sum);
+          }
+          sync();
         }
-        sync();
-      }
+      };
+      if (kg == 0) add(std::integral_constant<int, 0>());
+      else if (kg == 1) add(std::integral_constant<int, 1>());
+      else if (kg == 2) add(std::integral_constant<int, 2>());
+      else add(std::integral_constant<int, 3>());
       // ---- out, or to the block's workspace slot
       const bool whole = w.count == w.tiles;
       const int slot = dec::slot(w);
       for (int e = threadIdx.x; e < S::ROWS * (DP / 8); e += 32 * S::CONSUMERS) {
         const int r = e / (DP / 8), c = e % (DP / 8) * 8;
         if (r0 + r >= a.rows || c >= a.d) continue;
-        float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, m_sm[i * S::ROWS + r]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sum += mx == -INFINITY ? l_sm[i * S::ROWS + r] : exp2_sfu(m_sm[i * S::ROWS + r] - mx) * l_sm[i * S::ROWS + r];
+        const float2 ml = row_sm[r];
         const float* x0 = o_sm + r * S::OSTRIDE + c;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = x0[i];
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;  // a row that sees nothing is zero
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= inv;
           *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + dec::row_offset(a, w.b, w.head, r0 + r) + c) = pack8h(x, H16);
@@ -397,7 +419,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
           float* dst = a.part + ((int64_t)slot * S::ROWS + r) * a.d + c;
           *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
           *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
-          if (c == 0) a.part_ml[(int64_t)slot * S::ROWS + r] = make_float2(mx, sum);
+          if (c == 0) a.part_ml[(int64_t)slot * S::ROWS + r] = ml;
         }
       }
       if (threadIdx.x == 0) dec::note_segment(a, w);

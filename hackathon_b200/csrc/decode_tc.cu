@@ -120,32 +120,6 @@ __device__ __forceinline__ bool non_finite(const uint4& v, uint32_t inf) {
   return x;
 }
 
-// Which of the unit's 128 rows draft `tok` sees, as bits (before the scores are
-// in registers: 32 mask bytes are then on their way at a time).
-__device__ __forceinline__ void see(const Args& a, const dec::Walk& w, int tok, int key0, uint32_t* words) {
-  const int first = key0 - w.n;  // the unit's first row among the drafts; below 0: committed
-  const int drafts = w.end - w.n;
-  const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_stride + (int64_t)tok * a.tokens : nullptr;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t bits = 0;
-    if (first + 32 * i < drafts) {
-      uint8_t x[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const int j = first + 32 * i + c;
-        x[c] = mask ? mask[min(max(j, 0), a.tokens - 1)] : j <= tok;
-      }
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const int j = first + 32 * i + c;
-        bits |= (uint32_t)(j < 0 || (j < drafts && x[c] != 0)) << c;
-      }
-    }
-    words[i] = bits;
-  }
-}
-
 template <int DP, bool H16>
 __global__ void __launch_bounds__(THREADS, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
@@ -301,17 +275,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool live = r >= 0 && r0 + r < a.rows;
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int tok = live ? (r0 + r) / a.group : 0;
-      // ---- the row's queries (both groups share tile 0 when there is one: group i copies half of the dims)
+      // ---- the row's queries (both groups share tile 0 when there is one: group i brings half of the rows)
       {
         uint8_t* q_sm = sm + (two && grp ? S::TILE : 0);
-        const int qr = copy ? lane_row & 63 : lane_row;  // the query row at this row of the tile
-        const bool there = r0 + qr < a.rows;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                          (there ? dec::row_offset(a, w.b, w.head, r0 + qr) : 0));
-        const int c0 = two ? 0 : grp * (DP / 16), c1 = two ? DP / 8 : c0 + DP / 16;
+        // a warp's 32 rows of the tile, DP / 8 lanes side by side in a row
+        constexpr int PER = DP / 8, STEP = 32 / PER;
+        const int c = lane % PER;
+        const int i0 = two ? 0 : grp * 16, i1 = two ? 32 : i0 + 16;
 #pragma unroll 8
-        for (int c = c0; c < c1; ++c)
-          *reinterpret_cast<uint4*>(q_sm + at(lane_row, c)) = there && c * 8 < a.d ? src[c] : make_uint4(0, 0, 0, 0);
+        for (int i = i0; i < i1; i += STEP) {
+          const int row = (warp & 3) * 32 + i + lane / PER;
+          const int qr = r0 + (copy ? row & 63 : row);  // the query row at this row of the tile
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (qr < a.rows && c * 8 < a.d)
+            v = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + dec::row_offset(a, w.b, w.head, qr))[c];
+          *reinterpret_cast<uint4*>(q_sm + at(row, c)) = v;
+        }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -343,7 +322,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (warp_live) {
           uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
-          if (open) see(a, w, tok, key0, sees);
+          if (open) {  // before the scores are in registers: 32 mask bytes are on their way at a time
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sees[i] = dec::see<32>(a, w, tok, key0 + 32 * i);
+          }
           // the row's largest score; scores are read from TMEM twice, so that 64 at a time are in registers
           float top = -INFINITY;
 #pragma unroll 1
@@ -461,40 +443,43 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       const bool whole = w.count == w.tiles;
-      const int64_t slot_row = (int64_t)dec::slot(w) * (two ? 2 * ROWS : ROWS) + (two ? grp * ROWS : 0) + r;
+      const int64_t slot_row = (int64_t)dec::slot(w) * (two ? 2 * ROWS : ROWS) + (two ? grp * ROWS : 0);
+      // The warp's 32 rows pass through its part of the Q tile, 32 dims at a time, so that lanes side by side write
+      // neighbours: [32 rows][8 pieces of 4 dims], pieces turned by the row.
+      float4* stage = reinterpret_cast<float4*>(sm + (two && grp ? S::TILE : 0) + (warp & 3) * 4096);
+      const int row_base = (warp & 3) * 32;  // copies (up to 64 rows) are group 1's, which writes nothing
       // f: what the group's sums are multiplied by; `other`: group 1's rows in shared memory to add
       auto finish = [&](float f, float f_other, float mm, float ll, int c, float* o, const float4* other) {
-        if (!live) return;
-        if (other) {
+        const float inv = !whole ? 1.f : ll == 0.f ? 0.f : 1.f / ll;  // a row that sees nothing is zero
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 x = other[i * ROWS];
-            o[4 * i] = fmaf(o[4 * i], f, x.x * f_other);
-            o[4 * i + 1] = fmaf(o[4 * i + 1], f, x.y * f_other);
-            o[4 * i + 2] = fmaf(o[4 * i + 2], f, x.z * f_other);
-            o[4 * i + 3] = fmaf(o[4 * i + 3], f, x.w * f_other);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float4 x = other && live ? other[i * ROWS] : make_float4(0.f, 0.f, 0.f, 0.f);
+          stage[lane * 8 + (i ^ (lane & 7))] =
+              make_float4(fmaf(o[4 * i], f, x.x * f_other) * inv, fmaf(o[4 * i + 1], f, x.y * f_other) * inv,
+                          fmaf(o[4 * i + 2], f, x.z * f_other) * inv, fmaf(o[4 * i + 3], f, x.w * f_other) * inv);
         }
+        if (!whole && c == 0 && live) a.part_ml[slot_row + r] = make_float2(mm, ll);
+        __syncwarp();
         if (whole) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;  // a row that sees nothing is zero
-          uint16_t* dst = static_cast<uint16_t*>(a.out) + dec::row_offset(a, w.b, w.head, r0 + r) + c;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (c + 8 * i >= a.d) break;
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = o[8 * i + j] * inv;
-            reinterpret_cast<uint4*>(dst)[i] = pack8h(x, H16);
+            const int row = i * 8 + lane / 4, p = lane & 3;
+            const float4 u = stage[row * 8 + ((2 * p) ^ (row & 7))], v = stage[row * 8 + ((2 * p + 1) ^ (row & 7))];
+            const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            if (r0 + row_base + row < a.rows && c + 8 * p < a.d)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
+                                        dec::row_offset(a, w.b, w.head, r0 + row_base + row) + c + 8 * p) = pack8h(x, H16);
           }
         } else {
-          float* dst = a.part + slot_row * a.d + c;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (c + 4 * i >= a.d) break;
-            reinterpret_cast<float4*>(dst)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            const int row = i * 4 + lane / 8, p = lane & 7;
+            if (r0 + row_base + row < a.rows && c + 4 * p < a.d)
+              *reinterpret_cast<float4*>(a.part + (slot_row + row_base + row) * a.d + c + 4 * p) =
+                  stage[row * 8 + (p ^ (row & 7))];
           }
-          if (c == 0) a.part_ml[slot_row] = make_float2(mm, ll);
         }
+        __syncwarp();
       };
       auto load_o = [&](int c, float* o) {
         __syncwarp();  // the load is the warp's
