@@ -264,20 +264,6 @@ def launch(kid: int, ins: Sequence[Tensor], outs: Sequence[Tensor], params, stre
     check(L.c3b_launch(kid, ia, len(ins), oa, len(outs), pp, plen, C.c_void_p(stream)), f"{KERNEL_NAMES.get(kid, kid)}")
 
 
-_raw = None
-
-
-def launch_raw():
-    """c3b_launch taking the addresses of its tensor and parameter records."""
-    global _raw
-    if _raw is None:
-        fn = lib()["c3b_launch"]  # a function object of its own, with its own argument types
-        vp, i32 = C.c_void_p, C.c_int
-        fn.argtypes = [i32, vp, i32, vp, i32, vp, C.c_size_t, vp]
-        _raw = fn
-    return _raw
-
-
 def kernel_id(name: str) -> int:
     L = lib()
     rc = L.c3b_kernel_id(name.encode())

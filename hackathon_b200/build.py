@@ -22,6 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libc3b200.so"
+TORCH_SRC = CSRC / "torch_call.cpp"
+TORCH_LIB = PKG / "_torch_call.so"  # the fast calls from torch tensors; only where torch is installed
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -44,7 +46,43 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def _torch_dir():
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).parent if spec and spec.origin else None
+
+
+def torch_call_command(out: Path):
+    """g++ command of the torch binding, or None where torch or Python's headers are missing."""
+    import sysconfig
+    torch, python = _torch_dir(), Path(sysconfig.get_paths()["include"])
+    cxx = shutil.which("g++")
+    if torch is None or cxx is None or not (python / "Python.h").exists() or not (torch / "lib" / "libc10_cuda.so").exists():
+        return None
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    return [cxx, "-O2", "-std=c++20", "-shared", "-fPIC", "-w", str(TORCH_SRC), "-o", str(out), "-I", str(INCLUDE),
+            "-I", str(torch / "include"), "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"),
+            "-I", str(python), "-I", str(cuda), "-L", str(torch / "lib"), f"-Wl,-rpath,{torch / 'lib'}",
+            "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+
+
+def torch_call_needs_build() -> bool:
+    t = TORCH_LIB.stat().st_mtime if TORCH_LIB.exists() else -1.0
+    return any(p.stat().st_mtime > t for p in (TORCH_SRC, INCLUDE / "c3b200.h"))
+
+
+def build_torch_call(force: bool = False):
+    if not force and not torch_call_needs_build():
+        return
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    cmd = torch_call_command(tmp)
+    if cmd is not None:
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, TORCH_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_torch_call(force)
     if not force and not needs_build():
         return LIB
     objdir = ROOT / "_build"

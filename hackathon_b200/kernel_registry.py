@@ -202,87 +202,66 @@ for _name in _prepared_names():
 # checks, the parameter block, the tensor records) is kept for them; a call
 # fills in the addresses it was given.  Outputs have their own type and shape.
 
-_WORDS = C.sizeof(L.Tensor) // 8  # a tensor record in 8-byte words, its pointer first
-
-
-class _Ready:
-    __slots__ = ("kid", "n_in", "n_out", "records", "params", "plen", "workspace", "shapes")
-
-
-def _ready(name: str, inputs: List[Any], outputs: List[Any], params: Dict[str, Any]) -> _Ready:
+def _ready(name: str, inputs: List[Any], outputs: List[Any], params: Dict[str, Any]):
+    """What launches of this signature need: kernel id, inputs, tensor records (without addresses),
+    parameter block, bytes of a workspace to bring, and outputs given in another than their logical shape."""
     ins = [None if x is None else describe(x) for x in inputs]
     outs = [describe(o) for o in outputs]
-    r = _Ready()
-    r.workspace = 0
+    workspace = 0
     if name == "tree_attention" and len(outs) == 1 and len(ins) > 1 and \
             all(d is not None and len(d.shape) == 4 for d in ins[:2]):
-        r.workspace = tree_attention_workspace(ins[0], ins[1])
-        if r.workspace:
-            outs.append(Desc(0, L.U8, (r.workspace,)))
+        workspace = tree_attention_workspace(ins[0], ins[1])
+        if workspace:
+            outs.append(Desc(0, L.U8, (workspace,)))
     prep = prepare(name, ins, outs, params)
     ln, = prep.launches
-    r.kid, r.n_in, r.n_out, r.params, r.plen = ln.kid, len(ln.ins), len(ln.outs), ln.params, C.sizeof(ln.params)
-    r.records = bytes(L.tensor_array(ln.ins + ln.outs))
-    # outputs given flat come back in their logical shape
-    r.shapes = [(i, s) for i, s in enumerate(prep.out_shapes[:len(outputs)]) if tuple(outputs[i].shape) != tuple(s)]
-    return r
+    shapes = [(i, tuple(s)) for i, s in enumerate(prep.out_shapes[:len(outputs)]) if tuple(outputs[i].shape) != tuple(s)]
+    records = L.tensor_array(ln.ins + ln.outs)
+    for t in records:
+        t.ptr = None
+    return ln.kid, len(ln.ins), bytes(records), bytes(ln.params), workspace, shapes
+
+
+_torch_call = None  # the module, once it is bound to the kernel library; False where it was not built
+
+
+def _bound():
+    global _torch_call
+    if _torch_call is None:
+        try:
+            import torch  # noqa: F401  (its libraries are the module's)
+            from . import _torch_call as m
+        except ImportError:
+            _torch_call = False
+            return False
+        lib = L.lib()
+        m.bind(C.cast(lib.c3b_launch, C.c_void_p).value, C.cast(lib.c3b_last_error, C.c_void_p).value)
+        _torch_call = m
+    return _torch_call
 
 
 def _make_repeated(name: str) -> KernelFunc:
     generic = _make(name)
-    kept: Dict[Any, _Ready] = {}
+    state: List[Any] = []
 
-    def kernel(inputs: List[Any], outputs: List[Any], params: Dict[str, Any],
+    def kernel(inputs: List[Any], outputs: List[Any], params: Optional[Dict[str, Any]],
                tuning: Optional[Dict[str, int]] = None) -> None:
-        import torch
-        key: List[Any] = [len(inputs)]
-        ptrs: List[int] = []
-        dev = -1
-        for x in (*inputs, *outputs):
-            if x is None:
-                key.append(None)
-                continue
-            if not isinstance(x, torch.Tensor):
+        if state:
+            new = state[0].call(inputs, outputs, params)
+            if new is None:
+                return
+        else:
+            if not _bound():
                 return _with_workspace(generic, name, inputs, outputs, params)
-            if not x.is_contiguous():
-                raise ValueError("kernel arrays must be C-contiguous")
-            d = x.get_device()
-            if d != dev:
-                if d < 0:
-                    raise TypeError("kernel arrays must live on the GPU")
-                if dev >= 0:
-                    raise ValueError(f"{name}: arrays on different devices")
-                dev = d
-            key += (x.shape, x.dtype)
-            ptrs.append(x.data_ptr())
-        if dev < 0:
-            raise ValueError(f"{name}: no arrays")
-        if dev != torch._C._cuda_getDevice():
-            with torch.cuda.device(dev):
-                return kernel(inputs, outputs, params, tuning)
-        key.append(dev)
-        if params:
-            key += params.items()
-        signature = tuple(key)
-        r = kept.get(signature)
-        if r is None:
-            r = _ready(name, inputs, outputs, params or {})
-            if len(kept) >= 512:
-                kept.clear()
-            kept[signature] = r
-        n = r.n_in + r.n_out
-        if r.workspace:
-            scratch = torch.empty(r.workspace, dtype=torch.uint8, device=x.device)
-            ptrs.append(scratch.data_ptr())
-        records = (C.c_uint64 * (n * _WORDS)).from_buffer_copy(r.records)
-        records[0:n * _WORDS:_WORDS] = ptrs
-        at = C.addressof(records)
-        rc = L.launch_raw()(r.kid, at, r.n_in, at + r.n_in * _WORDS * 8, r.n_out, C.addressof(r.params), r.plen,
-                            torch._C._cuda_getCurrentRawStream(dev))
-        if rc < 0:
-            L.check(rc, name)
-        for i, shape in r.shapes:
-            outputs[i] = outputs[i].view(shape)
+            state.append(_torch_call.State(name))
+            new = state[0].call(inputs, outputs, params)
+        if isinstance(new, bytes):  # a signature seen for the first time: the checks
+            import torch
+            with torch.cuda.device(next(x for x in (*inputs, *outputs) if x is not None).device):
+                state[0].add(new, *_ready(name, inputs, outputs, params or {}))
+            new = state[0].call(inputs, outputs, params)
+        if new is NotImplemented:
+            _with_workspace(generic, name, inputs, outputs, params)
 
     kernel.__name__ = f"kernel_{name}"
     kernel.__qualname__ = kernel.__name__
