@@ -152,9 +152,9 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   int unit = 64, per_sm;
   if (f32) {
     pl.kernel = MMA32;
-    unit = 32;
     pl.rows = rows <= 16 || pl.dp == 256 ? 16 : 32;
-    per_sm = f32_blocks_per_sm(pl.dp, pl.rows);
+    unit = f32_unit(pl.dp, pl.rows);
+    per_sm = 1;
   } else if (pl.dp <= 128 && rows > 32) {
     // 33 to 128 rows: one tile for both softmax groups; more: a tile each
     pl.kernel = TC16;

@@ -217,7 +217,7 @@ int cache_maps(const Args& a, int box_rows, CUtensorMap* k, CUtensorMap* v);
 int mma_blocks_per_sm(int dp, int rows);
 int run_mma(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
 int run_tc(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
-int f32_blocks_per_sm(int dp, int rows);
+int f32_unit(int dp, int rows);
 int run_f32(const Plan& pl, const Args& a, cudaStream_t s);
 
 }  // namespace dec

@@ -1,13 +1,13 @@
 // fp32 attention of drafted tokens over a decoding cache, on tensor cores.
 //
-// The same operator, split, masks and block layout as decode_mma.cu, with units
-// of 32 cached rows (8 keys a warp).  Products are tf32 (mma.sync m16n8k8) on
-// operands split in two: x = hi + lo, each rounded to tf32's 11 bits, and
+// The same operator, split, masks and block layout as decode_mma.cu, with 8 keys
+// a warp.  Products are tf32 (mma.sync m16n8k8) on operands split in two:
+// x = hi + lo, each rounded to tf32's 11 bits, and
 //   x y = hi hi' + hi lo' + lo hi'   (lo lo' is below 2^-22 of the product),
 // each of the three with its own accumulators for the scores, which shortens
-// the chains and adds the small terms to each other first.  A cached row costs
-// 8 D bytes and three times the products, which stays below HBM's time up to 16
-// rows; in plain FMA the same rows would fill the FMA pipe.
+// the chains and adds the small terms to each other first.  Rounding to tf32 is
+// an integer addition and a mask.  Queries are split once a piece.  In plain FMA
+// 16 rows would fill the FMA pipe for longer than HBM needs.
 //
 // In P V the k index runs over the keys in the order 0 2 4 6 1 3 5 7: a thread's
 // score accumulators are then its weight operands as they stand, and the eight
@@ -25,8 +25,6 @@ namespace df32 {
 using namespace tc;
 using dec::Args;
 
-constexpr int KEYS = 32;
-
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -40,11 +38,13 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo, both in tf32.  Where x is not finite hi alone carries it.
+// x = hi + lo, both in tf32 (the products ignore the low 13 bits).  Where x is
+// not finite hi alone carries it.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) hi = __float_as_uint(x) | (x == x ? 0u : 0x400000u);
   const float rest = x - __uint_as_float(hi);
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest == rest ? rest : 0.f));
+  lo = __float_as_uint(rest == rest ? rest : 0.f) + 0x1000u;
 }
 
 // Byte offset of 16-byte chunk `ch` (4 dims) of row `row` in a tile of 128-byte
@@ -54,39 +54,39 @@ __device__ __forceinline__ uint32_t at(int row, int ch) {
   return (uint32_t)((ch >> 3) * (ROWS * 128) + row * 128 + (((ch ^ row) & 7) << 4));
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  MT: 16-row tiles.
-template <int DP, int MT>
+// DP: head_dim rounded up to 64, 128 or 256.  MT: 16-row tiles.  NW: consumer warps.
+template <int DP, int MT, int NW>
 struct Shape {
   static constexpr int ROWS = 16 * MT;
-  static constexpr int CONSUMERS = 4;
+  static constexpr int CONSUMERS = NW;
+  static constexpr int KEYS = 8 * NW;
   static constexpr int THREADS = 32 * (CONSUMERS + 1);
   static constexpr uint32_t TILE = KEYS * DP * 4;
   static constexpr int OSTRIDE = DP + 8;  // floats: fragment rows fall on different banks
   static constexpr uint32_t O_BYTES = (uint32_t)ROWS * OSTRIDE * 4;
-  static constexpr uint32_t Q_BYTES = (uint32_t)ROWS * DP * 4;
-  static constexpr uint32_t ML_BYTES = 2u * 5 * ROWS * 4;
+  static constexpr uint32_t Q_BYTES = 2u * ROWS * DP * 4;  // hi, lo
+  static constexpr uint32_t ML_BYTES = 2u * (NW + 1) * ROWS * 4;
   static constexpr uint32_t QO_BYTES = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;  // the sums are joined where Q stood
   static constexpr uint32_t REST = QO_BYTES + ML_BYTES + 256;
-  // two blocks an SM where both fit with three stages
-  static constexpr bool PAIR = 3 * 2 * TILE + REST + 1024 <= 113 * 1024;
-  static constexpr uint32_t BUDGET = (PAIR ? 113u : 226u) * 1024;
+  static constexpr uint32_t BUDGET = 226u * 1024;
   static constexpr int FIT = (int)((BUDGET - REST - 1024) / (2 * TILE));
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static_assert(STAGES >= 2, "a ring needs two stages");
   static constexpr uint32_t SMEM = STAGES * 2 * TILE + REST + 1024;
 };
 
-template <int DP, int MT>
-__global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR ? 2 : 1))
+template <int DP, int MT, int NW>
+__global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
     tree_f32_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
-  typedef Shape<DP, MT> S;
+  typedef Shape<DP, MT, NW> S;
+  constexpr int KEYS = S::KEYS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* q_sm = sm + S::STAGES * 2 * S::TILE;
   float* o_sm = reinterpret_cast<float*>(q_sm);
-  float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [4][ROWS]
-  float* l_sm = m_sm + 4 * S::ROWS;     // [4][ROWS]
-  float2* row_sm = reinterpret_cast<float2*>(l_sm + 4 * S::ROWS);  // [ROWS]
+  float* m_sm = reinterpret_cast<float*>(q_sm + S::QO_BYTES);  // [NW][ROWS]
+  float* l_sm = m_sm + NW * S::ROWS;     // [NW][ROWS]
+  float2* row_sm = reinterpret_cast<float2*>(l_sm + NW * S::ROWS);  // [ROWS]
   uint64_t* full = reinterpret_cast<uint64_t*>(row_sm + S::ROWS);
   uint64_t* empty = full + S::STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S::STAGES);
@@ -138,7 +138,10 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r0 + r < a.rows && ch * 4 < a.d)
           v = *reinterpret_cast<const float4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 4);
-        *reinterpret_cast<float4*>(q_sm + at<S::ROWS>(r, ch)) = v;
+        uint4 hi, lo;
+        split(v.x, hi.x, lo.x), split(v.y, hi.y, lo.y), split(v.z, hi.z, lo.z), split(v.w, hi.w, lo.w);
+        *reinterpret_cast<uint4*>(q_sm + at<S::ROWS>(r, ch)) = hi;
+        *reinterpret_cast<uint4*>(q_sm + S::ROWS * DP * 4 + at<S::ROWS>(r, ch)) = lo;
       }
       sync();
       const uint32_t q_base = smem_u32(q_sm);
@@ -173,10 +176,10 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t f[4], fh[4], fl[4];
-              ldsm4(q_base + at<S::ROWS>(qrow + 16 * i, 2 * (ks + h) + (lane >> 4)), f);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) split(__uint_as_float(f[c]), fh[c], fl[c]);
+              uint32_t fh[4], fl[4];
+              const uint32_t q_at = q_base + at<S::ROWS>(qrow + 16 * i, 2 * (ks + h) + (lane >> 4));
+              ldsm4(q_at, fh);
+              ldsm4(q_at + S::ROWS * DP * 4, fl);
               mma(acc[i][0], fh, bh[2 * h], bh[2 * h + 1]);
               mma(acc[i][1], fh, bl[2 * h], bl[2 * h + 1]);
               mma(acc[i][2], fl, bh[2 * h], bh[2 * h + 1]);
@@ -321,23 +324,25 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int r = 16 * i + 8 * half + g;
-          const float mx = fmaxf(fmaxf(m_sm[r], m_sm[S::ROWS + r]), fmaxf(m_sm[2 * S::ROWS + r], m_sm[3 * S::ROWS + r]));
+          float mx = m_sm[r];
+#pragma unroll
+          for (int k = 1; k < NW; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + r]);
           const float f = mx == -INFINITY ? 1.f : exp2f(m[i][half] - mx);
 #pragma unroll
           for (int nb = 0; nb < DP / 8; ++nb) o[i][nb][2 * half] *= f, o[i][nb][2 * half + 1] *= f;
         }
-      // In round k warp kg adds a quarter of the dims, quarter (kg + k) mod 4: always the same order, all warps at work.
+      // In round k warp kg adds part (kg + k) mod NW of the dims: always the same order, all warps at work.
       auto add = [&](auto me) {
         constexpr int KG = decltype(me)::value;
 #pragma unroll
-        for (int round = 0; round < 4; ++round) {
-          const int c = (KG + round) & 3;
+        for (int round = 0; round < NW; ++round) {
+          const int c = (KG + round) % NW;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-              for (int nb = c * (DP / 32); nb < (c + 1) * (DP / 32); ++nb) {
+              for (int nb = c * (DP / 8 / NW); nb < (c + 1) * (DP / 8 / NW); ++nb) {
                 float2* d = reinterpret_cast<float2*>(o_sm + (16 * i + 8 * half + g) * S::OSTRIDE + nb * 8 + 2 * t);
                 float2 x = make_float2(o[i][nb][2 * half], o[i][nb][2 * half + 1]);
                 if (round) {
@@ -350,9 +355,9 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             // the rows' maxima and sums over the four groups
             float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + lane]);
+            for (int k = 0; k < NW; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + lane]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < NW; ++k) {
               const float x = l_sm[k * S::ROWS + lane];
               sum += mx == -INFINITY ? x : exp2f(m_sm[k * S::ROWS + lane] - mx) * x;
             }
@@ -361,10 +366,19 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
           sync();
         }
       };
-      if (kg == 0) add(std::integral_constant<int, 0>());
-      else if (kg == 1) add(std::integral_constant<int, 1>());
-      else if (kg == 2) add(std::integral_constant<int, 2>());
-      else add(std::integral_constant<int, 3>());
+      switch (kg) {
+        case 0: add(std::integral_constant<int, 0>()); break;
+        case 1: add(std::integral_constant<int, 1>()); break;
+        case 2: add(std::integral_constant<int, 2>()); break;
+        case 3: add(std::integral_constant<int, 3>()); break;
+        default:
+          if constexpr (NW == 8) {
+            if (kg == 4) add(std::integral_constant<int, 4>());
+            else if (kg == 5) add(std::integral_constant<int, 5>());
+            else if (kg == 6) add(std::integral_constant<int, 6>());
+            else add(std::integral_constant<int, 7>());
+          }
+      }
       // ---- out, or to the block's workspace slot
       const bool whole = w.count == w.tiles;
       const int slot = dec::slot(w);
@@ -400,10 +414,10 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
   }
 }
 
-template <int DP, int MT>
+template <int DP, int MT, int NW>
 static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int grid, cudaStream_t s) {
-  typedef Shape<DP, MT> S;
-  auto kernel = tree_f32_kernel<DP, MT>;
+  typedef Shape<DP, MT, NW> S;
+  auto kernel = tree_f32_kernel<DP, MT, NW>;
   static std::atomic<uint64_t> done{0};
   if (int rc = dec::allow_smem(kernel, (int)S::SMEM, done)) return rc;
   return launch_pdl(kernel, grid, S::THREADS, (size_t)S::SMEM, s, km, vm, a);
@@ -413,20 +427,16 @@ static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int 
 
 namespace dec {
 
-int f32_blocks_per_sm(int dp, int rows) {
-  if (dp == 256) return df32::Shape<256, 1>::PAIR ? 2 : 1;
-  if (dp == 128) return (rows == 16 ? df32::Shape<128, 1>::PAIR : df32::Shape<128, 2>::PAIR) ? 2 : 1;
-  return (rows == 16 ? df32::Shape<64, 1>::PAIR : df32::Shape<64, 2>::PAIR) ? 2 : 1;
-}
+int f32_unit(int dp, int rows) { return dp == 64 || (dp == 128 && rows == 16) ? 64 : 32; }
 
 int run_f32(const Plan& pl, const Args& a, cudaStream_t s) {
   CUtensorMap km, vm;
-  if (int rc = cache_maps(a, df32::KEYS, &km, &vm)) return rc;
+  if (int rc = cache_maps(a, f32_unit(pl.dp, pl.rows), &km, &vm)) return rc;
   if (pl.dp == 64)
-    return pl.rows == 16 ? df32::run<64, 1>(km, vm, a, pl.grid, s) : df32::run<64, 2>(km, vm, a, pl.grid, s);
-  if (pl.dp == 128)
-    return pl.rows == 16 ? df32::run<128, 1>(km, vm, a, pl.grid, s) : df32::run<128, 2>(km, vm, a, pl.grid, s);
-  return df32::run<256, 1>(km, vm, a, pl.grid, s);
+    return pl.rows == 16 ? df32::run<64, 1, 8>(km, vm, a, pl.grid, s) : df32::run<64, 2, 8>(km, vm, a, pl.grid, s);
+  if (pl.dp == 128)  // 32 rows: twice the accumulators, so half the warps
+    return pl.rows == 16 ? df32::run<128, 1, 8>(km, vm, a, pl.grid, s) : df32::run<128, 2, 4>(km, vm, a, pl.grid, s);
+  return df32::run<256, 1, 4>(km, vm, a, pl.grid, s);
 }
 
 }  // namespace dec

@@ -101,108 +101,165 @@ __device__ __forceinline__ int64_t cache_row(const Args& a, int64_t b, int64_t t
   return n + t;
 }
 
-// A warp takes one token and chunk_heads of its heads; LPH lanes share a head,
-// each with a unit of 2 * VEC elements: VEC pairs, or 2 * VEC elements behind
-// the rotated part.  The sines of a lane's VEC pairs serve all heads of its
-// chunk.  NB heads are loaded before the first is stored.
-template <typename T, int VEC, int LPH, int NB>
-__global__ void __launch_bounds__(256) rotary_kernel(const Args a) {
+// Two values at a time, so that conversions and products come in pairs.
+template <typename T> __device__ __forceinline__ float2 pair_of(const T* v) { return make_float2(to_f32(v[0]), to_f32(v[1])); }
+template <> __device__ __forceinline__ float2 pair_of(const __nv_bfloat16* v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(v));
+}
+template <> __device__ __forceinline__ float2 pair_of(const __half* v) { return __half22float2(*reinterpret_cast<const __half2*>(v)); }
+template <typename T> __device__ __forceinline__ void set_pair(T* v, float2 x) { v[0] = x.x, v[1] = x.y; }
+template <> __device__ __forceinline__ void set_pair(__nv_bfloat16* v, float2 x) {
+  *reinterpret_cast<__nv_bfloat162*>(v) = __float22bfloat162_rn(x);
+}
+template <> __device__ __forceinline__ void set_pair(__half* v, float2 x) { *reinterpret_cast<__half2*>(v) = __float22half2_rn(x); }
+
+// What is done to a head besides the rotation.
+enum { PLAIN = 0, NORM = 1 /* weights shared by the heads, or none */, NORM_EACH = 2 /* weights of each head */ };
+
+// A warp takes one token and chunk_heads of its heads; `lanes` (a power of two)
+// lanes share a head, each with a unit of 2 * VEC elements: VEC pairs, or
+// 2 * VEC elements behind the rotated part.  A lane's sines, multiplied by the
+// norm's weights where all heads share them, serve every head of the chunk:
+//   a' = inv (a (w_a cos) - b (w_b sin)),  b' = inv (b (w_b cos) + a (w_a sin)).
+// NB heads are loaded before the first is stored.  HBM bounds it: 64 sequences of
+// 512 tokens, 32 + 16 heads of 128, bf16, 806 MB.
+template <typename T, int VEC, int MODE, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lanes) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, sub = lane % LPH;
-  constexpr int HPW = 32 / LPH;
-  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int64_t token = item / a.chunks;
+  constexpr int NB = 2;
+  const int lane = threadIdx.x & 31, sub = lane & (lanes - 1), hpw = 32 / lanes, own = lane / lanes;
+  const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+  const int token = item / a.chunks;
   if (token >= a.tokens) return;
-  const int64_t b = token / a.seq, t = token - b * a.seq;
-  const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
-  const int first = (int)(item - token * a.chunks) * a.chunk_heads;
-  const int last = min(total, first + a.chunk_heads);
-  const int rotated = a.rotary / (2 * VEC);
-  const bool active = sub < a.d / (2 * VEC), turned = sub < rotated;
+  const int b = token / a.seq, t = token - b * a.seq;
+  const int width = a.heads[0] + a.heads[1] + a.heads[2];
+  const int first = (item - token * a.chunks) * a.chunk_heads;
+  const int last = min(width - (a.copy_v ? 0 : a.heads[2]), first + a.chunk_heads);
+  const bool active = sub < a.d / (2 * VEC), turned = sub < a.rotary / (2 * VEC);
+  // the unit's two pieces: the two halves of its pairs, or two neighbours
+  const bool halves = !INTERLEAVED && turned;
+  const int off0 = halves ? sub * VEC : sub * 2 * VEC;
+  const int off1 = halves ? a.rotary / 2 + sub * VEC : off0 + VEC;
   float c[VEC], s[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) c[j] = 1.f, s[j] = 0.f;
   if (turned) {
     const long long pos = position(a, b, t);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) turn(pos, a.steps[sub * VEC + j], a.scale, c[j], s[j]);
   }
-  // the unit's two pieces: the two halves of its pairs, or two neighbours
-  const bool halves = turned && !a.interleaved;
-  const int off0 = halves ? sub * VEC : sub * 2 * VEC;
-  const int off1 = halves ? a.rotary / 2 + sub * VEC : off0 + VEC;
   const int64_t row = cache_row(a, b, t);
-  const T* src = static_cast<const T*>(a.in) + token * (int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) * a.d;
+  const T* src = static_cast<const T*>(a.in) + (int64_t)token * width * a.d;
 
-  for (int h0 = first; h0 < last; h0 += HPW * NB) {
-    Piece<T, VEC> p0[NB], p1[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int h = h0 + i * HPW + lane / LPH;
-      if (active && h < last) {
-        p0[i].load(src + (int64_t)h * a.d + off0);
-        p1[i].load(src + (int64_t)h * a.d + off1);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int h = h0 + i * HPW + lane / LPH;
-      if (h0 + i * HPW >= last) break;  // the same for the whole warp
-      const bool on = active && h < last;
-      const int role = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
-      const int hh = h - (role > 0 ? a.heads[0] : 0) - (role > 1 ? a.heads[1] : 0);
-      float x[VEC], y[VEC];
+#pragma unroll 1
+  for (int role = 0; role < 3; ++role) {
+    const int begin = role == 0 ? 0 : role == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
+    const int lo = max(first, begin), hi = min(last, begin + a.heads[role]);
+    if (lo >= hi) continue;
+    const bool split = role > 0 && a.lengths;  // k and v go into the caches
+    if (split && row < 0) continue;
+    T* dst = static_cast<T*>(a.out[role]) +
+             (split ? ((int64_t)b * a.heads[role] * a.capacity + row) * a.d : (int64_t)token * a.out_stride);
+    const int64_t pitch = split ? a.capacity * a.d : a.d;  // from a head to the next
+    // pair j: a' = a ca + b sb, b' = b cb + a sa
+    float ca[VEC], sb[VEC], cb[VEC], sa[VEC];
+    if (role < 2 && MODE != NORM_EACH) {
+      const float* w = MODE == NORM ? a.w[role] : nullptr;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        x[j] = on ? to_f32(p0[i].v[j]) : 0.f;
-        y[j] = on ? to_f32(p1[i].v[j]) : 0.f;
+        float wa = 1.f, wb = 1.f;
+        if (w && active) {
+          wa = INTERLEAVED ? w[off0 + 2 * j] : w[off0 + j];
+          wb = INTERLEAVED ? w[off0 + 2 * j + 1] : w[off1 + j];
+        }
+        ca[j] = wa * c[j], sb[j] = -wb * s[j], cb[j] = wb * c[j], sa[j] = wa * s[j];
       }
-      if (a.normalize) {
-        float q = 0.f;
+    }
+#pragma unroll 1
+    for (int h0 = lo; h0 < hi; h0 += hpw * NB) {
+      Piece<T, VEC> p0[NB], p1[NB];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) q = fmaf(x[j], x[j], fmaf(y[j], y[j], q));
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-        if (role < 2 && on) {
-          const float inv = rsqrtf(q / (float)a.d + a.eps);
-          const float* w = a.w[role];
-          if (w) w += (int64_t)hh * a.w_stride[role];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            x[j] *= w ? inv * w[off0 + j] : inv;
-            y[j] *= w ? inv * w[off1 + j] : inv;
-          }
+      for (int i = 0; i < NB; ++i) {
+        const int h = h0 + i * hpw + own;
+        if (active && h < hi) {
+          p0[i].load(src + (int64_t)h * a.d + off0);
+          p1[i].load(src + (int64_t)h * a.d + off1);
         }
       }
-      if (role < 2 && turned) {
-        if (a.interleaved) {
-          // pairs are neighbours: (x0, x1), (x2, x3), ... (y0, y1), ...
 #pragma unroll
-          for (int j = 0; j < VEC; j += 2) {
-            const float u = x[j], v = x[j + 1];
-            x[j] = u * c[j / 2] - v * s[j / 2];
-            x[j + 1] = v * c[j / 2] + u * s[j / 2];
-            const float m = y[j], n = y[j + 1];
-            y[j] = m * c[(VEC + j) / 2] - n * s[(VEC + j) / 2];
-            y[j + 1] = n * c[(VEC + j) / 2] + m * s[(VEC + j) / 2];
+      for (int i = 0; i < NB; ++i) {
+        const int h = h0 + i * hpw + own;
+        const bool on = active && h < hi;
+        T* to = dst + (h - begin) * pitch;
+        if (role < 2) {
+          // x, y: the pairs' first and second elements, two pairs at a time (half layout) or one pair (interleaved)
+          float2 x[VEC / 2], y[VEC / 2];
+#pragma unroll
+          for (int j = 0; j < VEC / 2; ++j) {
+            x[j] = pair_of(p0[i].v + 2 * j);
+            y[j] = pair_of(p1[i].v + 2 * j);
           }
-        } else {
+          float inv = 1.f;
+          if (MODE != PLAIN) {
+            float2 q = make_float2(0.f, 0.f);
+            if (on) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float u = x[j], v = y[j];
-            x[j] = u * c[j] - v * s[j];
-            y[j] = v * c[j] + u * s[j];
+              for (int j = 0; j < VEC / 2; ++j) {
+                q = __ffma2_rn(x[j], x[j], q);
+                q = __ffma2_rn(y[j], y[j], q);
+              }
+            }
+            float total = q.x + q.y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+              if (o < lanes) total += __shfl_xor_sync(0xffffffffu, total, o);
+            inv = rsqrtf(total / (float)a.d + a.eps);
+          }
+          if (MODE == NORM_EACH && on) {
+            const float* w = a.w[role];
+            if (w) w += (int64_t)(h - begin) * a.w_stride[role];
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              if (w) {
+                x[j] = __fmul2_rn(x[j], make_float2(w[off0 + 2 * j], w[off0 + 2 * j + 1]));
+                y[j] = __fmul2_rn(y[j], make_float2(w[off1 + 2 * j], w[off1 + 2 * j + 1]));
+              }
+            }
+          }
+          const float2 inv2 = make_float2(inv, inv);
+          auto A = [&](int j) { return MODE == NORM_EACH ? c[j] : ca[j]; };
+          auto B = [&](int j) { return MODE == NORM_EACH ? -s[j] : sb[j]; };
+          auto C = [&](int j) { return MODE == NORM_EACH ? c[j] : cb[j]; };
+          auto D = [&](int j) { return MODE == NORM_EACH ? s[j] : sa[j]; };
+#pragma unroll
+          for (int j = 0; j < VEC / 2; ++j) {
+            float2 u, v;
+            if (INTERLEAVED) {
+              // x[j] is pair j of the unit, y[j] pair VEC / 2 + j
+              const int k = VEC / 2 + j;
+              u = __fmul2_rn(x[j], make_float2(A(j), C(j)));
+              v = __fmul2_rn(y[j], make_float2(A(k), C(k)));
+              if (turned) {  // behind the rotated part nothing of a neighbour is added, not even 0 times it
+                u = __ffma2_rn(make_float2(x[j].y, x[j].x), make_float2(B(j), D(j)), u);
+                v = __ffma2_rn(make_float2(y[j].y, y[j].x), make_float2(B(k), D(k)), v);
+              }
+            } else {
+              u = __fmul2_rn(x[j], make_float2(A(2 * j), A(2 * j + 1)));
+              v = __fmul2_rn(y[j], make_float2(C(2 * j), C(2 * j + 1)));
+              if (turned) {
+                u = __ffma2_rn(y[j], make_float2(B(2 * j), B(2 * j + 1)), u);
+                v = __ffma2_rn(x[j], make_float2(D(2 * j), D(2 * j + 1)), v);
+              }
+            }
+            if (MODE != PLAIN) u = __fmul2_rn(u, inv2), v = __fmul2_rn(v, inv2);
+            set_pair(p0[i].v + 2 * j, u);
+            set_pair(p1[i].v + 2 * j, v);
           }
         }
-      }
-      T* dst = destination<T>(a, role, hh, token, b, row);
-      if (on && dst) {
-        Piece<T, VEC> o0, o1;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          o0.v[j] = from_f32<T>(x[j]);
-          o1.v[j] = from_f32<T>(y[j]);
+        if (on) {
+          p0[i].store(to + off0);
+          p1[i].store(to + off1);
         }
-        o0.store(dst + off0);
-        o1.store(dst + off1);
       }
     }
   }
@@ -251,29 +308,25 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const Args a) {
   for (int i = a.rotary + lane; i < a.d; i += 32) dst[i] = from_f32<T>(to_f32(src[i]) * (w ? inv * w[i] : inv));
 }
 
-template <typename T, int VEC, int LPH>
+template <typename T, int VEC>
 static int run(Args a, cudaStream_t s) {
-  constexpr int HPW = 32 / LPH, NB = 4;
+  const int units = a.d / (2 * VEC), lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32, hpw = 32 / lanes;
   const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
-  const int rounds = (total + HPW - 1) / HPW;
+  const int rounds = (total + hpw - 1) / hpw;
   // A warp keeps its sines for as many heads as it can; a token's heads are
   // split over warps only while the tokens alone are fewer than 32 warps an SM.
   const int64_t want = ((int64_t)sm_count() * 32 + a.tokens - 1) / a.tokens;
   const int chunks = (int)(want < rounds ? (want < 1 ? 1 : want) : rounds);
-  a.chunk_heads = (rounds + chunks - 1) / chunks * HPW;
+  a.chunk_heads = (rounds + chunks - 1) / chunks * hpw;
   a.chunks = (total + a.chunk_heads - 1) / a.chunk_heads;
-  const int64_t blocks = (a.tokens * a.chunks + 7) / 8;
-  C3B_REQUIRE(blocks < ((int64_t)1 << 31), "rotary: too many tokens");
-  return launch_pdl(rotary_kernel<T, VEC, LPH, NB>, (int)blocks, 256, 0, s, a);
-}
-
-template <typename T, int VEC>
-static int run_lanes(const Args& a, cudaStream_t s) {
-  const int units = a.d / (2 * VEC);
-  if (units <= 4) return run<T, VEC, 4>(a, s);
-  if (units <= 8) return run<T, VEC, 8>(a, s);
-  if (units <= 16) return run<T, VEC, 16>(a, s);
-  return run<T, VEC, 32>(a, s);
+  C3B_REQUIRE(a.tokens * a.chunks < ((int64_t)1 << 31) - 8, "rotary: too many tokens");
+  const int blocks = (int)((a.tokens * a.chunks + 7) / 8);
+  const int mode = !a.normalize ? PLAIN : a.w_stride[0] || a.w_stride[1] ? NORM_EACH : NORM;
+#define C3B_ROT(M)                                                                                     \
+  (a.interleaved ? launch_pdl(rotary_kernel<T, VEC, M, true>, blocks, 256, 0, s, a, lanes)              \
+                 : launch_pdl(rotary_kernel<T, VEC, M, false>, blocks, 256, 0, s, a, lanes))
+  return mode == PLAIN ? C3B_ROT(PLAIN) : mode == NORM ? C3B_ROT(NORM) : C3B_ROT(NORM_EACH);
+#undef C3B_ROT
 }
 
 template <typename T>
@@ -284,13 +337,13 @@ static int run_type(const Args& a, cudaStream_t s) {
   // head and every pointer, and leaves at most 32 units a head.
   uintptr_t at = (uintptr_t)a.in | (uintptr_t)a.out[0] | (uintptr_t)a.out[1] | (uintptr_t)a.out[2];
   auto fits = [&](int vec) {
-    return a.rotary % (2 * vec) == 0 && a.d % (2 * vec) == 0 && a.d <= 64 * vec && at % (vec * sizeof(T)) == 0;
+    return a.tokens < (1ll << 31) && a.rotary % (2 * vec) == 0 && a.d % (2 * vec) == 0 && a.d <= 64 * vec && at % (vec * sizeof(T)) == 0;
   };
   if constexpr (sizeof(T) == 2) {
-    if (fits(8)) return run_lanes<T, 8>(a, s);
+    if (fits(8)) return run<T, 8>(a, s);
   }
-  if (fits(4)) return run_lanes<T, 4>(a, s);
-  if (fits(2)) return run_lanes<T, 2>(a, s);
+  if (fits(4)) return run<T, 4>(a, s);
+  if (fits(2)) return run<T, 2>(a, s);
   const int64_t blocks = (a.tokens * total + 7) / 8;
   C3B_REQUIRE(blocks < ((int64_t)1 << 31), "rotary: too many heads");
   return launch_pdl(rotary_any_kernel<T>, (int)blocks, 256, 0, s, a);
