@@ -29,27 +29,30 @@ struct Args {
   int rtiles;            // row tiles of a kv head
   int split;             // 1: blocks share units evenly; 0: blocks take whole segments
   int min_units;         // units a block takes at least
+  int ahead;             // units that a segment counts for besides its own: what starting and ending a piece costs
   float scale_log2;
 };
 
 // How a call runs (host).
 struct Plan {
   int kernel;       // which of them
-  int dp, rows, rtiles, grid, split, min_units;
+  int dp, rows, rtiles, grid, split, min_units, ahead;
   int64_t segments;
   size_t part, part_ml, seg, bytes;  // workspace: offsets and size
 };
 
 // A block's way through its pieces.  A segment is one (sequence, kv head, row
 // tile); a piece is the part of a segment that the block has, units tile ..
-// tile + count - 1.  All counts fit 32 bits (checked at launch).
+// tile + count - 1 (count = 0: none, the block only has some of the units
+// `ahead` that the segment counts for).  All counts fit 32 bits (checked at
+// launch).
 struct Walk {
   int b, head, rtile;
   int n, end;       // committed rows; rows with the drafts (0, 0 where the sequence does not fit)
   int tiles;        // units of the segment
   int tile, count;
-  int left;         // units (split) or segments (not split) still to do, this piece included
-  int u;            // the piece's first unit among all of them
+  int left;         // units (split) or segments (not split) after this piece; -1: no more
+  int u, span;      // the segment's first unit among all of them, ahead included; the piece's end in the segment
   int share, extra; // units a block has: share + 1 for the first `extra` blocks, share for the others
   bool first;       // the block's first piece
 };
@@ -67,7 +70,14 @@ __device__ __forceinline__ void set_length(const Args& a, Walk& w, int n) {
 template <int UNIT>
 __device__ __forceinline__ int units_of(const Args& a, int n) {
   const bool fits = n >= 0 && n <= (int)a.capacity - a.tokens;
-  return max(1, fits ? (n + a.tokens + UNIT - 1) / UNIT : 0) * (a.kv_heads * a.rtiles);
+  return (a.ahead + max(1, fits ? (n + a.tokens + UNIT - 1) / UNIT : 0)) * (a.kv_heads * a.rtiles);
+}
+
+// The piece that begins `from` units into the segment, those ahead included.
+__device__ __forceinline__ void take(const Args& a, Walk& w, int from) {
+  w.span = min(a.ahead + w.tiles, from + w.left);
+  w.tile = max(from - a.ahead, 0);
+  w.count = max(w.span - a.ahead, 0) - w.tile;
 }
 
 // The block's first piece, with units of UNIT cached rows; every warp finds it
@@ -82,8 +92,8 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
     const int segments = a.batch * per;
     const int share = segments / (int)gridDim.x, extra = segments - share * (int)gridDim.x;
     const int s0 = (int)blockIdx.x * share + min((int)blockIdx.x, extra);
-    w.left = share + ((int)blockIdx.x < extra);
-    if (w.left <= 0) return w;
+    w.left = share + ((int)blockIdx.x < extra) - 1;
+    if (w.left < 0) return w;
     w.b = s0 / per;
     in_b = s0 - w.b * per;
     set_length<UNIT>(a, w, a.lengths[w.b]);
@@ -95,10 +105,11 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int blocks = min((int)gridDim.x, (sum + a.min_units - 1) / a.min_units);  // that have work
+    w.left = -1;
     if ((int)blockIdx.x >= blocks) return w;
     w.share = sum / blocks;
     w.extra = sum - w.share * blocks;
-    w.u = (int)blockIdx.x * w.share + min((int)blockIdx.x, w.extra);
+    const int u = (int)blockIdx.x * w.share + min((int)blockIdx.x, w.extra);
     w.left = w.share + ((int)blockIdx.x < w.extra);
     int before = 0;
     for (int i0 = 0;; i0 += 32) {
@@ -111,7 +122,7 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, before + x > w.u);
+      const unsigned past = __ballot_sync(0xffffffffu, before + x > u);
       if (past) {
         const int k = __ffs(past) - 1;
         w.b = i0 + k;
@@ -121,9 +132,10 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
       }
       before += __shfl_sync(0xffffffffu, x, 31);
     }
-    in_b = (w.u - before) / w.tiles;
-    w.tile = w.u - before - in_b * w.tiles;
-    w.count = min(w.tiles - w.tile, w.left);
+    in_b = (u - before) / (a.ahead + w.tiles);
+    w.u = before + in_b * (a.ahead + w.tiles);
+    take(a, w, u - w.u);
+    w.left -= w.span - (u - w.u);
   }
   w.head = a.rtiles == 1 ? in_b : in_b / a.rtiles;
   w.rtile = in_b - w.head * a.rtiles;
@@ -132,9 +144,11 @@ __device__ __forceinline__ Walk start(const Args& a, int lane) {
 
 template <int UNIT>
 __device__ __forceinline__ void next(const Args& a, Walk& w) {
-  w.left -= a.split ? w.count : 1;
-  if (w.left <= 0) return;
-  w.u += w.count;
+  if (w.left <= 0) {
+    w.left = -1;
+    return;
+  }
+  w.u += a.ahead + w.tiles;
   w.first = false;
   if (++w.rtile == a.rtiles) {
     w.rtile = 0;
@@ -144,8 +158,14 @@ __device__ __forceinline__ void next(const Args& a, Walk& w) {
       set_length<UNIT>(a, w, a.lengths[w.b]);
     }
   }
-  w.tile = 0;
-  w.count = a.split ? min(w.tiles, w.left) : w.tiles;
+  if (a.split) {
+    take(a, w, 0);
+    w.left -= w.span;
+  } else {
+    w.tile = 0;
+    w.count = w.tiles;
+    --w.left;
+  }
 }
 
 // The workspace slot of an unfinished piece: a block has one for the segment it
@@ -157,7 +177,7 @@ __device__ __forceinline__ int slot(const Walk& w) { return 2 * blockIdx.x + (w.
 __device__ __forceinline__ void note_segment(const Args& a, const Walk& w) {
   if (!a.split || w.tile != 0) return;
   const int64_t s = ((int64_t)w.b * a.kv_heads + w.head) * a.rtiles + w.rtile;
-  const int end = w.u + w.tiles - 1;  // the segment's last unit
+  const int end = w.u + a.ahead + w.tiles - 1;  // the segment's last unit
   const int large = w.extra * (w.share + 1);
   const int last = end < large ? end / (w.share + 1) : w.extra + (end - large) / w.share;
   a.segments[s] = w.count == w.tiles ? make_int2(-1, -1) : make_int2(slot(w), last);

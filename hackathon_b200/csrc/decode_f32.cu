@@ -108,7 +108,8 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
   if (warp == S::CONSUMERS) {
     if (lane == 0) {
       uint32_t it = 0;
-      for (; w.left > 0; dec::next<KEYS>(a, w)) {
+      for (; w.left >= 0; dec::next<KEYS>(a, w)) {
+        if (w.count == 0) continue;
         const int64_t row0 = ((int64_t)w.b * a.kv_heads + w.head) * a.capacity;
         for (int u = w.tile; u < w.tile + w.count; ++u, ++it) {
           const uint32_t st = it % S::STAGES;
@@ -129,7 +130,8 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
     const int g = lane >> 2, t = lane & 3;
     auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * S::CONSUMERS) : "memory"); };
     uint32_t it = 0;
-    for (; w.left > 0; dec::next<KEYS>(a, w)) {
+    for (; w.left >= 0; dec::next<KEYS>(a, w)) {
+      if (w.count == 0) continue;
       // ---- the piece's query rows: row r is token r / G, head r % G of the group
       const int r0 = w.rtile * S::ROWS;
       const float* q = static_cast<const float*>(a.q);

@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ------------------------------------------------ loads: K, V, K, V, ... of the block's units
       if (lane == 0) {
         uint32_t it = 0;
-        for (; w.left > 0; dec::next<KEYS>(a, w)) {
+        for (; w.left >= 0; dec::next<KEYS>(a, w)) {
+          if (w.count == 0) continue;
           const int64_t row0 = ((int64_t)w.b * a.kv_heads + w.head) * a.capacity;
           for (int u = w.tile; u < w.tile + w.count; ++u) {
 #pragma unroll
@@ -202,12 +203,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t pt[2] = {0, 0};
         bool ok = true;
         int piece = 0;
-        for (; w.left > 0 && ok; dec::next<KEYS>(a, w), ++piece) {
+        for (; w.left >= 0 && ok; dec::next<KEYS>(a, w)) {
+          if (w.count == 0) continue;
           const int n = w.count;
           const int steps = two ? n : (n + 1) / 2;
           // unit of group i's step k; >= n: none
           auto unit = [&](int i, int k) { return two ? k : 2 * k + i; };
-          if (!mbar_wait(q_full, piece & 1, abort_flag, 46)) break;
+          if (!mbar_wait(q_full, piece++ & 1, abort_flag, 46)) break;
           auto scores = [&](int i, int k) {
             const int u = unit(i, k);
             if (u >= n) return;
@@ -270,7 +272,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t t_s = tmem + lanes + COL_S + 128 * grp, t_o = tmem + lanes + COL_O + 128 * grp;
     constexpr uint32_t inf = H16 ? 0x7c00u : 0x7f80u;
     uint32_t ts = 0, to = 0, base = 0;
-    for (; w.left > 0; dec::next<KEYS>(a, w)) {
+    for (; w.left >= 0; dec::next<KEYS>(a, w)) {
+      if (w.count == 0) continue;
       const int r0 = w.rtile * (two ? 2 * ROWS : ROWS) + (two ? grp * ROWS : 0);
       const bool live = r >= 0 && r0 + r < a.rows;
       const bool warp_live = __any_sync(0xffffffffu, live);
