@@ -191,26 +191,34 @@ __device__ __forceinline__ bool visible(const Args& a, const Walk& w, int tok, i
   return a.mask ? a.mask[w.b * a.mask_stride + (int64_t)tok * a.tokens + j] != 0 : j <= tok;
 }
 
-// Which of cache rows key .. key + N - 1 draft `tok` sees, as bits.  The mask's
-// bytes are all in range and none waits for another.
+// Which of cache rows key .. key + N - 1 (N = 8, 16 or 32) the lane's draft `tok`
+// sees, as bits; the warp's drafts are tok of its lanes with `live` set.  Lanes
+// side by side read neighbouring bytes of the mask, 32 / N drafts at a time.
 template <int N>
-__device__ __forceinline__ uint32_t see(const Args& a, const Walk& w, int tok, int key) {
+__device__ __forceinline__ uint32_t see(const Args& a, const Walk& w, int tok, bool live, int key, int lane) {
+  constexpr uint32_t ALL = N == 32 ? ~0u : (1u << (N & 31)) - 1u;
   const int first = key - w.n;  // the first row among the drafts; below 0: committed
   const int drafts = w.end - w.n;
-  uint32_t bits = 0;
-  if (first < drafts) {
-    const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_stride + (int64_t)tok * a.tokens : nullptr;
-    uint8_t x[N];
-#pragma unroll
-    for (int c = 0; c < N; ++c) x[c] = first + c <= tok;
-    if (mask) {
-#pragma unroll
-      for (int c = 0; c < N; ++c) x[c] = mask[min(max(first + c, 0), a.tokens - 1)];
-    }
-#pragma unroll
-    for (int c = 0; c < N; ++c) bits |= (uint32_t)(first + c < 0 || (first + c < drafts && x[c] != 0)) << c;
+  const uint32_t committed = first >= 0 ? 0u : first <= -N ? ALL : (1u << -first) - 1u;
+  if (first >= drafts) return committed;
+  if (!a.mask) {
+    const int last = min(tok, drafts - 1) - first;  // of the N rows
+    return last < 0 ? committed : committed | (last >= N - 1 ? ALL : (2u << last) - 1u);
   }
-  return bits;
+  const uint8_t* mask = a.mask + w.b * a.mask_stride;
+  const int t0 = __reduce_min_sync(0xffffffffu, live ? tok : a.tokens);
+  const int t1 = __reduce_max_sync(0xffffffffu, live ? tok : -1);
+  const int j = first + lane % N;
+  const bool draft = j >= 0 && j < drafts;
+  uint32_t bits = 0;
+  constexpr int PER = 32 / N;
+#pragma unroll 4
+  for (int t = t0; t <= t1; t += PER) {
+    const int mine = t + lane / N;
+    const uint32_t seen = __ballot_sync(0xffffffffu, draft && mine <= t1 && mask[(int64_t)mine * a.tokens + j] != 0);
+    if (tok >= t && tok < t + PER) bits = seen >> ((tok - t) * N & 31);
+  }
+  return committed | (bits & ALL);
 }
 
 // Element offset, in q and the output, of query row r of a kv head.

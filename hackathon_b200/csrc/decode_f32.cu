@@ -135,15 +135,23 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
       // ---- the piece's query rows: row r is token r / G, head r % G of the group
       const int r0 = w.rtile * S::ROWS;
       const float* q = static_cast<const float*>(a.q);
-      for (int e = threadIdx.x; e < S::ROWS * (DP / 4); e += 32 * S::CONSUMERS) {
-        const int r = e / (DP / 4), ch = e % (DP / 4);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      constexpr int LOADS = S::ROWS * (DP / 4) / (32 * S::CONSUMERS);
+      float4 qv[LOADS];  // all on their way before the first is stored
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = threadIdx.x + i * 32 * S::CONSUMERS, r = e / (DP / 4), ch = e % (DP / 4);
+        qv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r0 + r < a.rows && ch * 4 < a.d)
-          v = *reinterpret_cast<const float4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 4);
+          qv[i] = *reinterpret_cast<const float4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = threadIdx.x + i * 32 * S::CONSUMERS;
+        const uint32_t to = at<S::ROWS>(e / (DP / 4), e % (DP / 4));
         uint4 hi, lo;
-        split(v.x, hi.x, lo.x), split(v.y, hi.y, lo.y), split(v.z, hi.z, lo.z), split(v.w, hi.w, lo.w);
-        *reinterpret_cast<uint4*>(q_sm + at<S::ROWS>(r, ch)) = hi;
-        *reinterpret_cast<uint4*>(q_sm + S::ROWS * DP * 4 + at<S::ROWS>(r, ch)) = lo;
+        split(qv[i].x, hi.x, lo.x), split(qv[i].y, hi.y, lo.y), split(qv[i].z, hi.z, lo.z), split(qv[i].w, hi.w, lo.w);
+        *reinterpret_cast<uint4*>(q_sm + to) = hi;
+        *reinterpret_cast<uint4*>(q_sm + S::ROWS * DP * 4 + to) = lo;
       }
       sync();
       const uint32_t q_base = smem_u32(q_sm);
@@ -196,9 +204,8 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         const bool open = key0 + 8 > w.n;  // the warp's keys reach past the committed rows
         bool poison = false;
         if (open) {
-          // a lane looks up a row's 8 keys, all its mask bytes at once
-          const int row = r0 + (lane & (S::ROWS - 1));
-          const uint32_t mine = dec::see<8>(a, w, row < a.rows ? row / a.group : 0, key0);
+          const int row = r0 + (lane & (S::ROWS - 1));  // whose keys the lane looks up
+          const uint32_t mine = dec::see<8>(a, w, row < a.rows ? row / a.group : 0, row < a.rows, key0, lane);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll

@@ -157,12 +157,19 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
       // ---- the piece's query rows: row r is token r / G, head r % G of the group
       const int r0 = w.rtile * S::ROWS;
       const uint16_t* q = static_cast<const uint16_t*>(a.q);
-      for (int e = threadIdx.x; e < S::ROWS * (DP / 8); e += 32 * S::CONSUMERS) {
-        const int r = e / (DP / 8), ch = e % (DP / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
+      constexpr int LOADS = S::ROWS * (DP / 8) / (32 * S::CONSUMERS);
+      uint4 qv[LOADS];  // all on their way before the first is stored
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = threadIdx.x + i * 32 * S::CONSUMERS, r = e / (DP / 8), ch = e % (DP / 8);
+        qv[i] = make_uint4(0, 0, 0, 0);
         if (r0 + r < a.rows && ch * 8 < a.d)
-          v = *reinterpret_cast<const uint4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 8);
-        *reinterpret_cast<uint4*>(q_sm + at<S::ROWS>(r, ch)) = v;
+          qv[i] = *reinterpret_cast<const uint4*>(q + dec::row_offset(a, w.b, w.head, r0 + r) + ch * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = threadIdx.x + i * 32 * S::CONSUMERS;
+        *reinterpret_cast<uint4*>(q_sm + at<S::ROWS>(e / (DP / 8), e % (DP / 8))) = qv[i];
       }
       sync();
       const uint32_t q_base = smem_u32(q_sm);
@@ -219,9 +226,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[i][nb][j] *= a.scale_log2;
         if (open) {
-          // a lane looks up a row's 16 keys, all its mask bytes at once
-          const int row = r0 + (lane & (S::ROWS - 1));
-          const uint32_t mine = dec::see<16>(a, w, row < a.rows ? row / a.group : 0, key0);
+          const int row = r0 + (lane & (S::ROWS - 1));  // whose keys the lane looks up
+          const uint32_t mine = dec::see<16>(a, w, row < a.rows ? row / a.group : 0, row < a.rows, key0, lane);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll

@@ -285,15 +285,20 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr int PER = DP / 8, STEP = 32 / PER;
         const int c = lane % PER;
         const int i0 = two ? 0 : grp * 16, i1 = two ? 32 : i0 + 16;
-#pragma unroll 8
-        for (int i = i0; i < i1; i += STEP) {
-          const int row = (warp & 3) * 32 + i + lane / PER;
+        // sixteen loads on their way before the first is stored
+        uint4 v[32 / STEP];
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; ++i) {
+          const int row = (warp & 3) * 32 + i * STEP + lane / PER;
           const int qr = r0 + (copy ? row & 63 : row);  // the query row at this row of the tile
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (qr < a.rows && c * 8 < a.d)
-            v = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + dec::row_offset(a, w.b, w.head, qr))[c];
-          *reinterpret_cast<uint4*>(q_sm + at(row, c)) = v;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (i * STEP >= i0 && i * STEP < i1 && qr < a.rows && c * 8 < a.d)
+            v[i] = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + dec::row_offset(a, w.b, w.head, qr))[c];
         }
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; ++i)
+          if (i * STEP >= i0 && i * STEP < i1)
+            *reinterpret_cast<uint4*>(q_sm + at((warp & 3) * 32 + i * STEP + lane / PER, c)) = v[i];
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -325,9 +330,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (warp_live) {
           uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
-          if (open) {  // before the scores are in registers: 32 mask bytes are on their way at a time
+          if (open) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sees[i] = dec::see<32>(a, w, tok, key0 + 32 * i);
+            for (int i = 0; i < 4; ++i) sees[i] = dec::see<32>(a, w, tok, live, key0 + 32 * i, lane);
           }
           // the row's largest score; scores are read from TMEM twice, so that 64 at a time are in registers
           float top = -INFINITY;
@@ -451,6 +456,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       // neighbours: [32 rows][8 pieces of 4 dims], pieces turned by the row.
       float4* stage = reinterpret_cast<float4*>(sm + (two && grp ? S::TILE : 0) + (warp & 3) * 4096);
       const int row_base = (warp & 3) * 32;  // copies (up to 64 rows) are group 1's, which writes nothing
+      int64_t out_at[4];  // elements of the output at the rows this lane writes
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = r0 + row_base + i * 8 + lane / 4;
+        out_at[i] = row < a.rows ? dec::row_offset(a, w.b, w.head, row) : -1;
+      }
       // f: what the group's sums are multiplied by; `other`: group 1's rows in shared memory to add
       auto finish = [&](float f, float f_other, float mm, float ll, int c, float* o, const float4* other) {
         const float inv = !whole ? 1.f : ll == 0.f ? 0.f : 1.f / ll;  // a row that sees nothing is zero
@@ -469,9 +480,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int row = i * 8 + lane / 4, p = lane & 3;
             const float4 u = stage[row * 8 + ((2 * p) ^ (row & 7))], v = stage[row * 8 + ((2 * p + 1) ^ (row & 7))];
             const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-            if (r0 + row_base + row < a.rows && c + 8 * p < a.d)
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
-                                        dec::row_offset(a, w.b, w.head, r0 + row_base + row) + c + 8 * p) = pack8h(x, H16);
+            if (out_at[i] >= 0 && c + 8 * p < a.d)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out_at[i] + c + 8 * p) = pack8h(x, H16);
           }
         } else {
 #pragma unroll
