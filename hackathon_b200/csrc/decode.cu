@@ -67,72 +67,97 @@ __global__ void __launch_bounds__(128) tree_rows_kernel(const Args a) {
   }
 }
 
-// Joins the parts of the segments that were split: a warp for each query row,
-// parts in block order.  At most 64 registers, so that its blocks fit beside the
-// attention kernel's and are there when that ends.  K: 128-dim halves of a head.
-template <int K>
+// Joins the parts of the segments that were split, in block order: a warp for RW
+// query rows of a segment.  At most 64 registers, so that its blocks fit beside
+// the attention kernel's and are there when that ends; what it costs is a chain
+// of three loads (segment, statistics, sums), so eight are on their way together.
+// K: 128-dim halves of a head.
+template <int K, int RW>
 __global__ void __launch_bounds__(256, 4) tree_join_kernel(const Args a, int tile_rows, int items) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   if (item >= items) return;
-  const int seg = item / tile_rows, r = item - seg * tile_rows;
-  const int bh = seg / a.rtiles, row = (seg - bh * a.rtiles) * tile_rows + r;
-  if (row >= a.rows) return;
+  const int per = tile_rows / RW, seg = item / per, r0 = (item - seg * per) * RW;
+  const int bh = seg / a.rtiles, row0 = (seg - bh * a.rtiles) * tile_rows + r0;
+  if (row0 >= a.rows) return;
   const int2 where = a.segments[seg];
   if (where.x < 0) return;
   const int first = where.x / 2, parts = where.y - first + 1;
-  auto slot = [&](int i) { return (int64_t)(i ? 2 * (first + i) : where.x) * tile_rows + r; };
-  // 32 parts at a time: their statistics a lane each, then their sums, several on their way together
-  float mx = -INFINITY, sum = 0.f;
-  float4 o[K];
+  // row r0 of part i's slot; rows past the last of the tile's are there, whatever they hold
+  auto slot = [&](int i) { return (int64_t)(i ? 2 * (first + i) : where.x) * tile_rows + r0; };
+  float mx[RW], sum[RW];
+  float4 o[RW][K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    const float2 ml = i0 + lane < parts ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-    const float top = fmaxf(mx, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
-    const float f = exp2f(ml.x - base), before = exp2f(mx - base);
-    mx = top;
-    sum = sum * before + f * ml.y;
+  for (int r = 0; r < RW; ++r) {
+    mx[r] = -INFINITY, sum[r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) o[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i0 = 0; i0 < parts; i0 += 32) {  // 32 parts at a time, their statistics a lane each
+    float f[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const bool on = i0 + lane < parts && row0 + r < a.rows;
+      const float2 ml = on ? a.part_ml[slot(i0 + lane) + r] : make_float2(-INFINITY, 0.f);
+      const float top = fmaxf(mx[r], warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
+      const float before = exp2f(mx[r] - base);
+      f[r] = exp2f(ml.x - base);
+      mx[r] = top;
+      sum[r] = sum[r] * before + f[r] * ml.y;
+#pragma unroll
+      for (int k = 0; k < K; ++k) o[r][k].x *= before, o[r][k].y *= before, o[r][k].z *= before, o[r][k].w *= before;
+    }
     const int here = min(32, parts - i0);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      constexpr int NB = 8 / K;
-      o[k].x *= before, o[k].y *= before, o[k].z *= before, o[k].w *= before;
-      const int c = 4 * lane + 128 * k;
+    constexpr int NB = 8 / (K * RW);
 #pragma unroll 1
-      for (int i = 0; i < here; i += NB) {
-        float4 x[NB];
+    for (int i = 0; i < here; i += NB) {
+      float4 x[NB][RW][K];
 #pragma unroll
-        for (int q = 0; q < NB; ++q)
-          if (c < a.d && i + q < here) x[q] = *reinterpret_cast<const float4*>(a.part + slot(i0 + i + q) * a.d + c);
+      for (int q = 0; q < NB; ++q)
 #pragma unroll
-        for (int q = 0; q < NB; ++q) {
-          const float fi = __shfl_sync(0xffffffffu, f, i + q);
-          if (c < a.d && i + q < here) {
-            o[k].x = fmaf(fi, x[q].x, o[k].x);
-            o[k].y = fmaf(fi, x[q].y, o[k].y);
-            o[k].z = fmaf(fi, x[q].z, o[k].z);
-            o[k].w = fmaf(fi, x[q].w, o[k].w);
+        for (int r = 0; r < RW; ++r)
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const int c = 4 * lane + 128 * k;
+            x[q][r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < a.d && i + q < here && row0 + r < a.rows)
+              x[q][r][k] = *reinterpret_cast<const float4*>(a.part + (slot(i0 + i + q) + r) * a.d + c);
+          }
+#pragma unroll
+      for (int q = 0; q < NB; ++q)
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const float fi = __shfl_sync(0xffffffffu, f[r], i + q);
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            o[r][k].x = fmaf(fi, x[q][r][k].x, o[r][k].x);
+            o[r][k].y = fmaf(fi, x[q][r][k].y, o[r][k].y);
+            o[r][k].z = fmaf(fi, x[q][r][k].z, o[r][k].z);
+            o[r][k].w = fmaf(fi, x[q][r][k].w, o[r][k].w);
           }
         }
-      }
     }
   }
-  sum = warp_sum(sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t at = row_offset(a, bh / a.kv_heads, bh % a.kv_heads, row);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = 4 * lane + 128 * k;
-    if (c >= a.d) break;
-    const float x[4] = {o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv};
-    if (a.dtype == C3B_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + c) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-      const bool h16 = a.dtype == C3B_F16;
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at + c) =
-          make_uint2(pack2h(make_float2(x[0], x[1]), h16), pack2h(make_float2(x[2], x[3]), h16));
+  for (int r = 0; r < RW; ++r) {
+    const float total = warp_sum(sum[r]);
+    if (row0 + r >= a.rows) continue;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int64_t at = row_offset(a, bh / a.kv_heads, bh % a.kv_heads, row0 + r);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = 4 * lane + 128 * k;
+      if (c >= a.d) break;
+      const float4 x = make_float4(o[r][k].x * inv, o[r][k].y * inv, o[r][k].z * inv, o[r][k].w * inv);
+      if (a.dtype == C3B_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + c) = x;
+      } else {
+        const bool h16 = a.dtype == C3B_F16;
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at + c) =
+            make_uint2(pack2h(make_float2(x.x, x.y), h16), pack2h(make_float2(x.z, x.w), h16));
+      }
     }
   }
 }
@@ -148,6 +173,7 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
       (int64_t)p.batch * p.kv_heads * p.capacity >= (1ll << 31))
     return pl;
   const int64_t rows = (int64_t)p.tokens * (p.heads / p.kv_heads);
+  if (rows >= 1 << 20) return pl;  // token_of()
   pl.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
   int unit = 64, per_sm;
   if (f32) {
@@ -200,6 +226,7 @@ struct CommitArgs {
 template <typename W>
 __global__ void __launch_bounds__(128) commit_kernel(const CommitArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (item >= (int64_t)a.batch * a.kv_heads * 2) return;
@@ -288,6 +315,7 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
   a.batch = p.batch, a.tokens = p.tokens, a.heads = p.heads, a.kv_heads = p.kv_heads, a.d = p.head_dim;
   a.group = p.heads / p.kv_heads;
   a.rows = p.tokens * a.group;
+  a.inv_group = 1.f / (float)a.group;
   a.dtype = q.dtype;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   const uintptr_t at = (uintptr_t)q.ptr | (uintptr_t)k.ptr | (uintptr_t)v.ptr | (uintptr_t)out[0].ptr;
@@ -310,8 +338,11 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
     if (int rc = pl.kernel == MMA32 ? run_f32(pl, a, s) : pl.kernel == TC16 ? run_tc(h16, pl, a, s) : run_mma(h16, pl, a, s))
       return rc;
     if (!pl.split) return C3B_OK;
-    const int items = (int)pl.segments * pl.rows;
-    return launch_pdl(p.head_dim <= 128 ? tree_join_kernel<1> : tree_join_kernel<2>, (items + 7) / 8, 256, 0, s, a, pl.rows, items);
+    // four rows a warp once one a warp would take several rounds of the GPU
+    const int rw = p.head_dim <= 128 && pl.segments * pl.rows > 64ll * sm_count() ? 4 : 1;
+    const int items = (int)(pl.segments * pl.rows / rw);
+    auto join = p.head_dim > 128 ? tree_join_kernel<2, 1> : rw == 4 ? tree_join_kernel<1, 4> : tree_join_kernel<1, 1>;
+    return launch_pdl(join, (items + 7) / 8, 256, 0, s, a, pl.rows, items);
   }
   return launch_pdl(tree_rows_kernel, (int)rows, 128, 0, s, a);
 }

@@ -30,7 +30,7 @@ struct Args {
   int split;             // 1: blocks share units evenly; 0: blocks take whole segments
   int min_units;         // units a block takes at least
   int ahead;             // units that a segment counts for besides its own: what starting and ending a piece costs
-  float scale_log2;
+  float scale_log2, inv_group;
 };
 
 // How a call runs (host).
@@ -221,9 +221,12 @@ __device__ __forceinline__ uint32_t see(const Args& a, const Walk& w, int tok, b
   return committed | (bits & ALL);
 }
 
+// The draft of query row r: r / group.  Rows are below 2^20, so (r + 1/2) / group is off by less than the 1/2.
+__device__ __forceinline__ int token_of(const Args& a, int r) { return (int)(((float)r + 0.5f) * a.inv_group); }
+
 // Element offset, in q and the output, of query row r of a kv head.
 __device__ __forceinline__ int64_t row_offset(const Args& a, int b, int head, int r) {
-  const int tok = r / a.group;
+  const int tok = token_of(a, r);
   return (((int64_t)b * a.tokens + tok) * a.heads + head * a.group + (r - tok * a.group)) * a.d;
 }
 

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         bool poison = false;
         if (open) {
           const int row = r0 + (lane & (S::ROWS - 1));  // whose keys the lane looks up
-          const uint32_t mine = dec::see<8>(a, w, row < a.rows ? row / a.group : 0, row < a.rows, key0, lane);
+          const uint32_t mine = dec::see<8>(a, w, row < a.rows ? dec::token_of(a, row) : 0, row < a.rows, key0, lane);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll

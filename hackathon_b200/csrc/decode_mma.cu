@@ -227,7 +227,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             for (int j = 0; j < 4; ++j) s[i][nb][j] *= a.scale_log2;
         if (open) {
           const int row = r0 + (lane & (S::ROWS - 1));  // whose keys the lane looks up
-          const uint32_t mine = dec::see<16>(a, w, row < a.rows ? row / a.group : 0, row < a.rows, key0, lane);
+          const uint32_t mine = dec::see<16>(a, w, row < a.rows ? dec::token_of(a, row) : 0, row < a.rows, key0, lane);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll

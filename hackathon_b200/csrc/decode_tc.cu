@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int r0 = w.rtile * (two ? 2 * ROWS : ROWS) + (two ? grp * ROWS : 0);
       const bool live = r >= 0 && r0 + r < a.rows;
       const bool warp_live = __any_sync(0xffffffffu, live);
-      const int tok = live ? (r0 + r) / a.group : 0;
+      const int tok = live ? dec::token_of(a, r0 + r) : 0;
       // ---- the row's queries (both groups share tile 0 when there is one: group i brings half of the rows)
       {
         uint8_t* q_sm = sm + (two && grp ? S::TILE : 0);

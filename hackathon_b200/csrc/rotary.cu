@@ -126,6 +126,7 @@ enum { PLAIN = 0, NORM = 1 /* weights shared by the heads, or none */, NORM_EACH
 template <typename T, int VEC, int MODE, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lanes) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int NB = 2;
   const int lane = threadIdx.x & 31, sub = lane & (lanes - 1), hpw = 32 / lanes, own = lane / lanes;
   const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_any_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
   const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
