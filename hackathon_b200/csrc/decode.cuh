@@ -5,8 +5,6 @@
 
 #include <cuda.h>
 
-#include <atomic>
-
 #include "common.cuh"
 
 namespace c3b {
@@ -228,19 +226,6 @@ __device__ __forceinline__ int token_of(const Args& a, int r) { return (int)(((f
 __device__ __forceinline__ int64_t row_offset(const Args& a, int b, int head, int r) {
   const int tok = token_of(a, r);
   return (((int64_t)b * a.tokens + tok) * a.heads + head * a.group + (r - tok * a.group)) * a.d;
-}
-
-// Dynamic shared memory above 48 KB, allowed once for each kernel and device.
-template <typename K>
-inline int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  C3B_CHECK_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(done.load(std::memory_order_relaxed) & bit)) {
-    C3B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.fetch_or(bit, std::memory_order_relaxed);
-  }
-  return C3B_OK;
 }
 
 // Tensor maps of the caches: rows of all heads one below the other, boxes of 128 bytes and `box_rows` rows.

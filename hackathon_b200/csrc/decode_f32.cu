@@ -428,7 +428,7 @@ static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int 
   typedef Shape<DP, MT, NW> S;
   auto kernel = tree_f32_kernel<DP, MT, NW>;
   static std::atomic<uint64_t> done{0};
-  if (int rc = dec::allow_smem(kernel, (int)S::SMEM, done)) return rc;
+  if (int rc = allow_smem(kernel, (int)S::SMEM, done)) return rc;
   return launch_pdl(kernel, grid, S::THREADS, (size_t)S::SMEM, s, km, vm, a);
 }
 

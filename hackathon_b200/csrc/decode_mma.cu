@@ -445,7 +445,7 @@ static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int 
   typedef Shape<DP, MT> S;
   auto kernel = tree_mma_kernel<DP, MT, H16>;
   static std::atomic<uint64_t> done{0};
-  if (int rc = dec::allow_smem(kernel, (int)S::SMEM, done)) return rc;
+  if (int rc = allow_smem(kernel, (int)S::SMEM, done)) return rc;
   return launch_pdl(kernel, grid, S::THREADS, (size_t)S::SMEM, s, km, vm, a);
 }
 

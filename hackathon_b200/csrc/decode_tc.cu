@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 template <int DP, bool H16>
 static int run(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int grid, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = dec::allow_smem(tree_tc_kernel<DP, H16>, (int)Shape<DP>::SMEM, done)) return rc;
+  if (int rc = allow_smem(tree_tc_kernel<DP, H16>, (int)Shape<DP>::SMEM, done)) return rc;
   return launch_pdl(tree_tc_kernel<DP, H16>, grid, THREADS, (size_t)Shape<DP>::SMEM, s, km, vm, a);
 }
 

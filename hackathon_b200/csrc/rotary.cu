@@ -14,6 +14,7 @@
 // no cosine table to read.  The upper 32 bits of the phase go to sincospif.
 //
 // Everything is computed in fp32 and rounded once, to the output's type.
+#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
@@ -39,7 +40,7 @@ struct Args {
   int seq, heads[3], d, rotary, pos64, interleaved, normalize, copy_v;
   int64_t out_stride;   // elements from one token to the next in out[0] (and in out[1], out[2] without lengths)
   int chunks, chunk_heads;
-  float scale, eps;
+  float scale, eps, inv_d;
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -116,19 +117,166 @@ template <> __device__ __forceinline__ void set_pair(__half* v, float2 x) { *rei
 // What is done to a head besides the rotation.
 enum { PLAIN = 0, NORM = 1 /* weights shared by the heads, or none */, NORM_EACH = 2 /* weights of each head */ };
 
-// A warp takes one token and chunk_heads of its heads; `lanes` (a power of two)
-// lanes share a head, each with a unit of 2 * VEC elements: VEC pairs, or
-// 2 * VEC elements behind the rotated part.  A lane's sines, multiplied by the
-// norm's weights where all heads share them, serve every head of the chunk:
+// A lane's part in the heads of one token: a unit of 2 * VEC elements, VEC pairs
+// or 2 * VEC elements behind the rotated part.  LANES lanes (a power of two; 0:
+// known at run time) share a head, and the heads of a warp share the work on the
+// sines.  These, multiplied by the norm's weights where all heads
+// share them, serve every head:
 //   a' = inv (a (w_a cos) - b (w_b sin)),  b' = inv (b (w_b cos) + a (w_a sin)).
-// NB heads are loaded before the first is stored.  HBM bounds it: 64 sequences of
-// 512 tokens, 32 + 16 heads of 128, bf16, 806 MB.
+template <typename T, int VEC, int MODE, bool INTERLEAVED, int LANES>
+struct Unit {
+  int sub, off0, off1;  // the unit's two pieces of VEC elements
+  bool active, turned;
+  int lanes, own, role; // own: which head of the warp's; role: whose coefficients are held, -1: none
+  float c[VEC], s[VEC];
+  float ca[VEC], sb[VEC], cb[VEC], sa[VEC];  // pair j: a' = a ca + b sb, b' = b cb + a sa
+
+  __device__ __forceinline__ Unit(const Args& a, int lane, int lanes_) {
+    lanes = LANES ? LANES : lanes_;
+    sub = lane & (lanes - 1), own = lane / lanes;
+    active = sub < a.d / (2 * VEC), turned = sub < a.rotary / (2 * VEC);
+    // a piece of each half of the rotated part, or of each half of what is behind it: lanes side by side, pieces too
+    off0 = turned ? sub * VEC : a.rotary / 2 + sub * VEC;
+    off1 = off0 + (turned ? a.rotary : a.d - a.rotary) / 2;
+  }
+
+  // The frequency of pair j: (off0 + j, off1 + j), or, interleaved, one of the pairs within the pieces.
+  __device__ __forceinline__ int pair_index(const Args& a, int j) const {
+    return !INTERLEAVED ? sub * VEC + j : j < VEC / 2 ? sub * (VEC / 2) + j : a.rotary / 4 + sub * (VEC / 2) + j - VEC / 2;
+  }
+
+  __device__ __forceinline__ void set_token(const Args& a, int b, int t) {
+    role = -1;
+    const long long pos = position(a, b, t);
+    if constexpr (LANES > 0) {
+      // pair i * SHARE + g of the unit is worked out by the warp's head g
+      constexpr int SHARE = 32 / LANES < VEC ? 32 / LANES : VEC;
+#pragma unroll
+      for (int i = 0; i < VEC / SHARE; ++i) {
+        float x, y;
+        turn(pos, a.steps[turned ? pair_index(a, i * SHARE + own % SHARE) : 0], a.scale, x, y);
+#pragma unroll
+        for (int g = 0; g < SHARE; ++g) {
+          c[i * SHARE + g] = __shfl_sync(0xffffffffu, x, sub + g * LANES);
+          s[i * SHARE + g] = __shfl_sync(0xffffffffu, y, sub + g * LANES);
+        }
+      }
+    } else if (turned) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) turn(pos, a.steps[pair_index(a, j)], a.scale, c[j], s[j]);
+    }
+    if (!turned) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) c[j] = 1.f, s[j] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void set_role(const Args& a, int r) {
+    if (r == role || r == 2) return;
+    role = r;
+    if (MODE == NORM_EACH) return;
+    const float* w = MODE == NORM ? a.w[r] : nullptr;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float wa = 1.f, wb = 1.f;
+      if (w && active) {
+        const float* pair = j < VEC / 2 ? w + off0 + 2 * j : w + off1 + 2 * j - VEC;
+        wa = INTERLEAVED ? pair[0] : w[off0 + j];
+        wb = INTERLEAVED ? pair[1] : w[off1 + j];
+      }
+      ca[j] = wa * c[j], sb[j] = -wb * s[j], cb[j] = wb * c[j], sa[j] = wa * s[j];
+    }
+  }
+
+  // Head h of the q (r = 0) or k (r = 1) heads, in place; the whole warp calls, `on` where the lane has a part.
+  __device__ __forceinline__ void head(const Args& a, int r, int h, bool on, Piece<T, VEC>& p0, Piece<T, VEC>& p1) const {
+    // two pairs at a time (half layout) or one (interleaved)
+    float2 x[VEC / 2], y[VEC / 2];
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      x[j] = pair_of(p0.v + 2 * j);
+      y[j] = pair_of(p1.v + 2 * j);
+    }
+    float inv = 1.f;
+    if (MODE != PLAIN) {
+      float2 q = make_float2(0.f, 0.f);
+      if (on) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          q = __ffma2_rn(x[j], x[j], q);
+          q = __ffma2_rn(y[j], y[j], q);
+        }
+      }
+      float total = q.x + q.y;
+      if constexpr (LANES > 0) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      } else {
+        for (int o = lanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      }
+      inv = rsqrtf(fmaf(total, a.inv_d, a.eps));
+    }
+    if (MODE == NORM_EACH && on) {
+      const float* w = a.w[r];
+      if (w) {
+        w += (int64_t)h * a.w_stride[r];
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          x[j] = __fmul2_rn(x[j], make_float2(w[off0 + 2 * j], w[off0 + 2 * j + 1]));
+          y[j] = __fmul2_rn(y[j], make_float2(w[off1 + 2 * j], w[off1 + 2 * j + 1]));
+        }
+      }
+    }
+    const float2 inv2 = make_float2(inv, inv);
+    auto A = [&](int j) { return MODE == NORM_EACH ? c[j] : ca[j]; };
+    auto B = [&](int j) { return MODE == NORM_EACH ? -s[j] : sb[j]; };
+    auto C = [&](int j) { return MODE == NORM_EACH ? c[j] : cb[j]; };
+    auto D = [&](int j) { return MODE == NORM_EACH ? s[j] : sa[j]; };
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      float2 u, v;
+      if (INTERLEAVED) {
+        // x[j] is pair j of the unit, y[j] pair VEC / 2 + j
+        const int k = VEC / 2 + j;
+        u = __fmul2_rn(x[j], make_float2(A(j), C(j)));
+        v = __fmul2_rn(y[j], make_float2(A(k), C(k)));
+        if (turned) {  // behind the rotated part nothing of a neighbour is added, not even 0 times it
+          u = __ffma2_rn(make_float2(x[j].y, x[j].x), make_float2(B(j), D(j)), u);
+          v = __ffma2_rn(make_float2(y[j].y, y[j].x), make_float2(B(k), D(k)), v);
+        }
+      } else {
+        u = __fmul2_rn(x[j], make_float2(A(2 * j), A(2 * j + 1)));
+        v = __fmul2_rn(y[j], make_float2(C(2 * j), C(2 * j + 1)));
+        if (turned) {
+          u = __ffma2_rn(y[j], make_float2(B(2 * j), B(2 * j + 1)), u);
+          v = __ffma2_rn(x[j], make_float2(D(2 * j), D(2 * j + 1)), v);
+        }
+      }
+      if (MODE != PLAIN) u = __fmul2_rn(u, inv2), v = __fmul2_rn(v, inv2);
+      set_pair(p0.v + 2 * j, u);
+      set_pair(p1.v + 2 * j, v);
+    }
+  }
+};
+
+// Where a role's heads of the token go, and how far one is from the next; null: nowhere.
+template <typename T>
+__device__ __forceinline__ T* heads_of(const Args& a, int role, int token, int b, int64_t row, int64_t& pitch) {
+  const bool cached = role > 0 && a.lengths;
+  pitch = cached ? a.capacity * a.d : a.d;
+  if (cached && row < 0) return nullptr;
+  return static_cast<T*>(a.out[role]) +
+         (cached ? ((int64_t)b * a.heads[role] * a.capacity + row) * a.d : (int64_t)token * a.out_stride);
+}
+
+// Narrower pieces than 16 bytes, or weights of each head: a warp takes one token and
+// chunk_heads of its heads; NB heads are loaded before the first is stored.
 template <typename T, int VEC, int MODE, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lanes) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int NB = 2;
-  const int lane = threadIdx.x & 31, sub = lane & (lanes - 1), hpw = 32 / lanes, own = lane / lanes;
+  const int lane = threadIdx.x & 31, hpw = 32 / lanes, own = lane / lanes;
   const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   const int token = item / a.chunks;
   if (token >= a.tokens) return;
@@ -136,134 +284,154 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
   const int width = a.heads[0] + a.heads[1] + a.heads[2];
   const int first = (item - token * a.chunks) * a.chunk_heads;
   const int last = min(width - (a.copy_v ? 0 : a.heads[2]), first + a.chunk_heads);
-  const bool active = sub < a.d / (2 * VEC), turned = sub < a.rotary / (2 * VEC);
-  // the unit's two pieces: the two halves of its pairs, or two neighbours
-  const bool halves = !INTERLEAVED && turned;
-  const int off0 = halves ? sub * VEC : sub * 2 * VEC;
-  const int off1 = halves ? a.rotary / 2 + sub * VEC : off0 + VEC;
-  float c[VEC], s[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) c[j] = 1.f, s[j] = 0.f;
-  if (turned) {
-    const long long pos = position(a, b, t);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) turn(pos, a.steps[sub * VEC + j], a.scale, c[j], s[j]);
-  }
+  Unit<T, VEC, MODE, INTERLEAVED, 0> unit(a, lane, lanes);
+  unit.set_token(a, b, t);
   const int64_t row = cache_row(a, b, t);
   const T* src = static_cast<const T*>(a.in) + (int64_t)token * width * a.d;
-
+  int begin = 0;
 #pragma unroll 1
-  for (int role = 0; role < 3; ++role) {
-    const int begin = role == 0 ? 0 : role == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
+  for (int role = 0; role < 3; begin += a.heads[role], ++role) {
     const int lo = max(first, begin), hi = min(last, begin + a.heads[role]);
-    if (lo >= hi) continue;
-    const bool split = role > 0 && a.lengths;  // k and v go into the caches
-    if (split && row < 0) continue;
-    T* dst = static_cast<T*>(a.out[role]) +
-             (split ? ((int64_t)b * a.heads[role] * a.capacity + row) * a.d : (int64_t)token * a.out_stride);
-    const int64_t pitch = split ? a.capacity * a.d : a.d;  // from a head to the next
-    // pair j: a' = a ca + b sb, b' = b cb + a sa
-    float ca[VEC], sb[VEC], cb[VEC], sa[VEC];
-    if (role < 2 && MODE != NORM_EACH) {
-      const float* w = MODE == NORM ? a.w[role] : nullptr;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float wa = 1.f, wb = 1.f;
-        if (w && active) {
-          wa = INTERLEAVED ? w[off0 + 2 * j] : w[off0 + j];
-          wb = INTERLEAVED ? w[off0 + 2 * j + 1] : w[off1 + j];
-        }
-        ca[j] = wa * c[j], sb[j] = -wb * s[j], cb[j] = wb * c[j], sa[j] = wa * s[j];
-      }
-    }
+    int64_t pitch;
+    T* dst = heads_of<T>(a, role, token, b, row, pitch);
+    if (lo >= hi || !dst) continue;
+    unit.set_role(a, role);
 #pragma unroll 1
     for (int h0 = lo; h0 < hi; h0 += hpw * NB) {
       Piece<T, VEC> p0[NB], p1[NB];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int h = h0 + i * hpw + own;
-        if (active && h < hi) {
-          p0[i].load(src + (int64_t)h * a.d + off0);
-          p1[i].load(src + (int64_t)h * a.d + off1);
+        if (unit.active && h < hi) {
+          p0[i].load(src + (int64_t)h * a.d + unit.off0);
+          p1[i].load(src + (int64_t)h * a.d + unit.off1);
         }
       }
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const int h = h0 + i * hpw + own;
-        const bool on = active && h < hi;
-        T* to = dst + (h - begin) * pitch;
-        if (role < 2) {
-          // x, y: the pairs' first and second elements, two pairs at a time (half layout) or one pair (interleaved)
-          float2 x[VEC / 2], y[VEC / 2];
-#pragma unroll
-          for (int j = 0; j < VEC / 2; ++j) {
-            x[j] = pair_of(p0[i].v + 2 * j);
-            y[j] = pair_of(p1[i].v + 2 * j);
-          }
-          float inv = 1.f;
-          if (MODE != PLAIN) {
-            float2 q = make_float2(0.f, 0.f);
-            if (on) {
-#pragma unroll
-              for (int j = 0; j < VEC / 2; ++j) {
-                q = __ffma2_rn(x[j], x[j], q);
-                q = __ffma2_rn(y[j], y[j], q);
-              }
-            }
-            float total = q.x + q.y;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-              if (o < lanes) total += __shfl_xor_sync(0xffffffffu, total, o);
-            inv = rsqrtf(total / (float)a.d + a.eps);
-          }
-          if (MODE == NORM_EACH && on) {
-            const float* w = a.w[role];
-            if (w) w += (int64_t)(h - begin) * a.w_stride[role];
-#pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) {
-              if (w) {
-                x[j] = __fmul2_rn(x[j], make_float2(w[off0 + 2 * j], w[off0 + 2 * j + 1]));
-                y[j] = __fmul2_rn(y[j], make_float2(w[off1 + 2 * j], w[off1 + 2 * j + 1]));
-              }
-            }
-          }
-          const float2 inv2 = make_float2(inv, inv);
-          auto A = [&](int j) { return MODE == NORM_EACH ? c[j] : ca[j]; };
-          auto B = [&](int j) { return MODE == NORM_EACH ? -s[j] : sb[j]; };
-          auto C = [&](int j) { return MODE == NORM_EACH ? c[j] : cb[j]; };
-          auto D = [&](int j) { return MODE == NORM_EACH ? s[j] : sa[j]; };
-#pragma unroll
-          for (int j = 0; j < VEC / 2; ++j) {
-            float2 u, v;
-            if (INTERLEAVED) {
-              // x[j] is pair j of the unit, y[j] pair VEC / 2 + j
-              const int k = VEC / 2 + j;
-              u = __fmul2_rn(x[j], make_float2(A(j), C(j)));
-              v = __fmul2_rn(y[j], make_float2(A(k), C(k)));
-              if (turned) {  // behind the rotated part nothing of a neighbour is added, not even 0 times it
-                u = __ffma2_rn(make_float2(x[j].y, x[j].x), make_float2(B(j), D(j)), u);
-                v = __ffma2_rn(make_float2(y[j].y, y[j].x), make_float2(B(k), D(k)), v);
-              }
-            } else {
-              u = __fmul2_rn(x[j], make_float2(A(2 * j), A(2 * j + 1)));
-              v = __fmul2_rn(y[j], make_float2(C(2 * j), C(2 * j + 1)));
-              if (turned) {
-                u = __ffma2_rn(y[j], make_float2(B(2 * j), B(2 * j + 1)), u);
-                v = __ffma2_rn(x[j], make_float2(D(2 * j), D(2 * j + 1)), v);
-              }
-            }
-            if (MODE != PLAIN) u = __fmul2_rn(u, inv2), v = __fmul2_rn(v, inv2);
-            set_pair(p0[i].v + 2 * j, u);
-            set_pair(p1[i].v + 2 * j, v);
-          }
-        }
+        const int h = h0 + i * hpw + own - begin;
+        const bool on = unit.active && h + begin < hi;
+        if (role < 2) unit.head(a, role, h, on, p0[i], p1[i]);
         if (on) {
-          p0[i].store(to + off0);
-          p1[i].store(to + off1);
+          p0[i].store(dst + h * pitch + unit.off0);
+          p1[i].store(dst + h * pitch + unit.off1);
         }
       }
     }
   }
+}
+
+// The common case, 16-byte pieces.  HBM bounds it, so the loads need no
+// registers: a warp brings its heads, which lie side by side, into shared memory
+// by bulk copies of up to PIECE bytes of q, k or v heads, STAGES ahead of its
+// work, across tokens.  A warp takes items (a token and chunk_heads of its
+// heads) W apart.
+constexpr int WARPS = 8, STAGES = 3, PIECE = 4096;
+constexpr uint32_t BULK_SMEM = WARPS * STAGES * PIECE;
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+
+template <typename T, int MODE, bool INTERLEAVED, int LANES>
+__global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a, const int items) {
+  constexpr int VEC = 16 / sizeof(T), HPW = 32 / LANES;
+  extern __shared__ __align__(128) uint8_t ring_sm[];
+  __shared__ uint64_t bars[WARPS][STAGES];
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = ring_sm + warp * (STAGES * PIECE);
+  uint64_t* full = bars[warp];
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int k0 = a.heads[0], v0 = k0 + a.heads[1], width = v0 + a.heads[2], total = a.copy_v ? width : v0;
+  const int per = PIECE / (a.d * (int)sizeof(T)) / HPW * HPW;  // heads of a piece, at most
+  const int step = (int)gridDim.x * WARPS;
+  // heads of the piece that begins at head h of a chunk that ends at `last`: all q, all k or all v
+  auto heads_from = [&](int h, int last) { return min(per, min(last, h < k0 ? k0 : h < v0 ? v0 : width) - h); };
+
+  // the next piece to bring: an item, and a head
+  int next_item = (int)blockIdx.x * WARPS + warp, next_head = -1, next_last = 0;
+  const T* next_src = nullptr;
+  auto bring = [&](int st) {
+    if (next_item >= items) return;
+    if (next_head < 0) {
+      const int token = next_item / a.chunks;
+      next_head = (next_item - token * a.chunks) * a.chunk_heads;
+      next_last = min(total, next_head + a.chunk_heads);
+      next_src = static_cast<const T*>(a.in) + (int64_t)token * width * a.d;
+    }
+    const int n = heads_from(next_head, next_last);
+    if (lane == 0) {
+      const uint32_t bytes = (uint32_t)(n * a.d * (int)sizeof(T));
+      tc::mbar_arrive_tx(&full[st], bytes);
+      bulk_load(ring + st * PIECE, next_src + next_head * a.d, bytes, &full[st]);
+    }
+    next_head += n;
+    if (next_head >= next_last) next_head = -1, next_item += step;
+  };
+  for (int i = 0; i < STAGES; ++i) bring(i);
+
+  Unit<T, VEC, MODE, INTERLEAVED, LANES> unit(a, lane, LANES);
+  int st = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int item = (int)blockIdx.x * WARPS + warp; item < items && ok; item += step) {
+    const int token = item / a.chunks, first = (item - token * a.chunks) * a.chunk_heads;
+    const int last = min(total, first + a.chunk_heads);
+    const int b = token / a.seq, t = token - b * a.seq;
+    unit.set_token(a, b, t);
+    const int64_t row = cache_row(a, b, t);
+    for (int h0 = first; h0 < last;) {
+      const int n = heads_from(h0, last);
+      const int role = h0 < k0 ? 0 : h0 < v0 ? 1 : 2, head = h0 - (role == 0 ? 0 : role == 1 ? k0 : v0);
+      h0 += n;
+      if (!tc::mbar_wait(&full[st], phase, &abort_flag, 51)) {
+        ok = false;
+        break;
+      }
+      int64_t pitch;
+      T* dst = heads_of<T>(a, role, token, b, row, pitch);
+      if (dst) {
+        unit.set_role(a, role);
+        dst += (head + unit.own) * pitch;
+        const T* src = reinterpret_cast<const T*>(ring + st * PIECE) + unit.own * a.d;
+        if (role == 2) {
+#pragma unroll 2
+          for (int h = unit.own; h < n; h += HPW, src += HPW * a.d, dst += HPW * pitch) {
+            if (!unit.active) continue;
+            Piece<T, VEC> p0, p1;
+            p0.load(src + unit.off0), p1.load(src + unit.off1);
+            p0.store(dst + unit.off0), p1.store(dst + unit.off1);
+          }
+        } else {
+#pragma unroll 2
+          for (int h = 0; h < n; h += HPW, src += HPW * a.d, dst += HPW * pitch) {
+            const bool on = unit.active && h + unit.own < n;
+            Piece<T, VEC> p0, p1;
+            if (on) p0.load(src + unit.off0), p1.load(src + unit.off1);
+            unit.head(a, role, 0, on, p0, p1);
+            if (on) p0.store(dst + unit.off0), p1.store(dst + unit.off1);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the piece
+      bring(st);
+      if (++st == STAGES) st = 0, phase ^= 1;
+    }
+  }
+  if (!ok)  // copies still in flight land before the block's shared memory is given back
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
 
 // Any even rotary size, head size and alignment: a warp per head, one pair a lane.
@@ -310,29 +478,56 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const Args a) {
   for (int i = a.rotary + lane; i < a.d; i += 32) dst[i] = from_f32<T>(to_f32(src[i]) * (w ? inv * w[i] : inv));
 }
 
+template <typename T, int MODE, bool INTERLEAVED, int LANES>
+static int launch_bulk(const Args& a, int items, cudaStream_t s) {
+  const int blocks = (items + WARPS - 1) / WARPS, most = 2 * sm_count();  // two an SM are resident
+  auto kernel = rotary_bulk_kernel<T, MODE, INTERLEAVED, LANES>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_smem(kernel, (int)BULK_SMEM, done)) return rc;
+  return launch_pdl(kernel, blocks < most ? blocks : most, 32 * WARPS, BULK_SMEM, s, a, items);
+}
+
+template <typename T, int VEC, int MODE, bool INTERLEAVED>
+static int launch(const Args& a, int lanes, int items, cudaStream_t s) {
+  if constexpr (VEC * sizeof(T) == 16 && MODE != NORM_EACH) {
+    switch (lanes) {
+      case 4: return launch_bulk<T, MODE, INTERLEAVED, 4>(a, items, s);
+      case 8: return launch_bulk<T, MODE, INTERLEAVED, 8>(a, items, s);
+      case 16: return launch_bulk<T, MODE, INTERLEAVED, 16>(a, items, s);
+      default: return launch_bulk<T, MODE, INTERLEAVED, 32>(a, items, s);
+    }
+  } else {
+    return launch_pdl(rotary_kernel<T, VEC, MODE, INTERLEAVED>, (items + 7) / 8, 256, 0, s, a, lanes);
+  }
+}
+
 template <typename T, int VEC>
 static int run(Args a, cudaStream_t s) {
   const int units = a.d / (2 * VEC), lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32, hpw = 32 / lanes;
   const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
   const int rounds = (total + hpw - 1) / hpw;
-  // A warp keeps its sines for as many heads as it can; a token's heads are
-  // split over warps only while the tokens alone are fewer than 32 warps an SM.
-  const int64_t want = ((int64_t)sm_count() * 32 + a.tokens - 1) / a.tokens;
-  const int chunks = (int)(want < rounds ? (want < 1 ? 1 : want) : rounds);
-  a.chunk_heads = (rounds + chunks - 1) / chunks * hpw;
+  // A token's heads are split over warps where that shortens the way of the
+  // longest warp: waves of 16 warps an SM, each as long as its rounds of heads
+  // and about three more for the token's positions and sines.
+  const int64_t wave = (int64_t)sm_count() * 16;
+  int64_t best = 0;
+  for (int chunks = 1; chunks <= rounds && chunks <= 64; ++chunks) {
+    const int each = (rounds + chunks - 1) / chunks;
+    const int64_t cost = (a.tokens * chunks + wave - 1) / wave * (each + 3);
+    if (chunks == 1 || cost < best) best = cost, a.chunk_heads = each * hpw;
+  }
   a.chunks = (total + a.chunk_heads - 1) / a.chunk_heads;
   C3B_REQUIRE(a.tokens * a.chunks < ((int64_t)1 << 31) - 8, "rotary: too many tokens");
-  const int blocks = (int)((a.tokens * a.chunks + 7) / 8);
+  const int items = (int)(a.tokens * a.chunks);
   const int mode = !a.normalize ? PLAIN : a.w_stride[0] || a.w_stride[1] ? NORM_EACH : NORM;
-#define C3B_ROT(M)                                                                                     \
-  (a.interleaved ? launch_pdl(rotary_kernel<T, VEC, M, true>, blocks, 256, 0, s, a, lanes)              \
-                 : launch_pdl(rotary_kernel<T, VEC, M, false>, blocks, 256, 0, s, a, lanes))
+#define C3B_ROT(M) (a.interleaved ? launch<T, VEC, M, true>(a, lanes, items, s) : launch<T, VEC, M, false>(a, lanes, items, s))
   return mode == PLAIN ? C3B_ROT(PLAIN) : mode == NORM ? C3B_ROT(NORM) : C3B_ROT(NORM_EACH);
 #undef C3B_ROT
 }
 
 template <typename T>
-static int run_type(const Args& a, cudaStream_t s) {
+static int run_type(Args a, cudaStream_t s) {
+  a.inv_d = 1.f / (float)a.d;
   const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0);
   if (a.tokens == 0 || total == 0 || a.d == 0) return C3B_OK;
   // Widest piece (16, 8 or 4 bytes) that divides the rotated part's halves, the

@@ -8,6 +8,7 @@
 
 #include <cuda.h>
 
+#include <atomic>
 #include <cstdlib>
 
 #include "common.cuh"
@@ -402,6 +403,19 @@ inline int launch_pdl_cluster(Kern kernel, int grid, int cluster, int block, siz
   cfg.attrs = at;
   cfg.numAttrs = pdl ? 2 : 1;
   C3B_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return C3B_OK;
+}
+
+// Dynamic shared memory above 48 KB, allowed once for each kernel and device.
+template <typename K>
+inline int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  C3B_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    C3B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
   return C3B_OK;
 }
 
