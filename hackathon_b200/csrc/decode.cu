@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256, 4) tree_join_kernel(const Args a, int til
 
 // The kernel that takes a call of these sizes: whole 16-byte pieces of a head,
 // and cache rows that TMA's 32-bit coordinates reach; else tree_rows_kernel.
-enum { ROWS_ANY = 0, MMA16, TC16, MMA32 };
+enum { ROWS_ANY = 0, MMA16, TC16, MMA32, SIMT32 };
 
 static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   Plan pl = {};
@@ -176,7 +176,12 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   if (rows >= 1 << 20) return pl;  // token_of()
   pl.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
   int unit = 64, per_sm;
-  if (f32) {
+  if (f32 && rows <= 8) {
+    pl.kernel = SIMT32;
+    pl.rows = rows <= 4 ? 4 : 8;
+    unit = simt_unit(pl.dp);
+    per_sm = 1;
+  } else if (f32) {
     pl.kernel = MMA32;
     pl.rows = rows <= 16 || pl.dp == 256 ? 16 : 32;
     unit = f32_unit(pl.dp, pl.rows);
@@ -335,7 +340,10 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
     a.min_units = pl.min_units;
     a.ahead = pl.split ? pl.ahead : 0;
     const bool h16 = q.dtype == C3B_F16;
-    if (int rc = pl.kernel == MMA32 ? run_f32(pl, a, s) : pl.kernel == TC16 ? run_tc(h16, pl, a, s) : run_mma(h16, pl, a, s))
+    if (int rc = pl.kernel == SIMT32  ? run_simt(pl, a, s)
+                 : pl.kernel == MMA32 ? run_f32(pl, a, s)
+                 : pl.kernel == TC16  ? run_tc(h16, pl, a, s)
+                                      : run_mma(h16, pl, a, s))
       return rc;
     if (!pl.split) return C3B_OK;
     // four rows a warp once one a warp would take several rounds of the GPU

@@ -1,5 +1,5 @@
 // What the attention kernels over a decoding cache share (decode.cu, decode_mma.cu,
-// decode_tc.cu, decode_f32.cu):
+// decode_tc.cu, decode_f32.cu, decode_simt.cu):
 // arguments, the split of the work over blocks, and the walk of a block over its pieces.
 #pragma once
 
@@ -235,6 +235,8 @@ int run_mma(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
 int run_tc(bool h16, const Plan& pl, const Args& a, cudaStream_t s);
 int f32_unit(int dp, int rows);
 int run_f32(const Plan& pl, const Args& a, cudaStream_t s);
+int simt_unit(int dp);
+int run_simt(const Plan& pl, const Args& a, cudaStream_t s);
 
 }  // namespace dec
 }  // namespace c3b

@@ -26,25 +26,29 @@ using namespace tc;
 using dec::Args;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+  asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo, both in tf32 (the products ignore the low 13 bits).  Where x is
-// not finite hi alone carries it.
+// ldmatrix and the products are not volatile, so that the compiler may overlap
+// them; pinned registers keep them in their place: a stage's address is pinned
+// after the wait for its data, the sums before its release.
+__device__ __forceinline__ void pin(uint32_t& x) { asm volatile("" : "+r"(x) : : "memory"); }
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x) : : "memory"); }
+
+// x = hi + lo for tf32 products, which ignore the low 13 bits: hi is x rounded to
+// the 11 that count, lo the rest, of which they see 11 more.  Where x is infinite
+// hi alone carries it.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) hi = __float_as_uint(x) | (x == x ? 0u : 0x400000u);
-  const float rest = x - __uint_as_float(hi);
-  lo = __float_as_uint(rest == rest ? rest : 0.f) + 0x1000u;
+  lo = fabsf(x) == INFINITY ? 0u : __float_as_uint(x - __uint_as_float(hi));
 }
 
 // Byte offset of 16-byte chunk `ch` (4 dims) of row `row` in a tile of 128-byte
@@ -154,7 +158,8 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         *reinterpret_cast<uint4*>(q_sm + S::ROWS * DP * 4 + to) = lo;
       }
       sync();
-      const uint32_t q_base = smem_u32(q_sm);
+      uint32_t q_base = smem_u32(q_sm);
+      pin(q_base);
       const int qrow = (lane & 7) + ((lane >> 3) & 1) * 8;
       float o[MT][DP / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
@@ -169,7 +174,8 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         const uint32_t st = it % S::STAGES;
         mbar_wait(&full[st], (it / S::STAGES) & 1, abort_flag, 44);  // on expiry every wait returns: all warps finish
         uint8_t* v_sm = sm + st * 2 * S::TILE + S::TILE;
-        const uint32_t k_base = smem_u32(sm + st * 2 * S::TILE);
+        uint32_t k_base = smem_u32(sm + st * 2 * S::TILE);
+        pin(k_base);
         // ---- S = Q K^T for the warp's 8 keys: hi hi', hi lo', lo hi'
         float s[MT][4], acc[MT][3][4];
 #pragma unroll
@@ -312,6 +318,12 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
             }
           }
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int nb = 0; nb < DP / 8; ++nb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pin(o[i][nb][j]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }

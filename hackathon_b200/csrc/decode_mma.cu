@@ -44,30 +44,34 @@ using dec::Args;
 constexpr int KEYS = 64;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+  asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+  asm("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 template <bool H16>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (H16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+// ldmatrix and the products are not volatile, so that the compiler may overlap
+// them; pinned registers keep them in their place: a stage's address is pinned
+// after the wait for its data, the sums before its release.
+__device__ __forceinline__ void pin(uint32_t& x) { asm volatile("" : "+r"(x) : : "memory"); }
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x) : : "memory"); }
 
 // Byte offset of 16-byte chunk `ch` of row `row` in a tile of 128-byte rows
 // (64 dims) under the 128-byte swizzle; further dims follow in tiles of ROWS rows.
@@ -172,7 +176,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
         *reinterpret_cast<uint4*>(q_sm + at<S::ROWS>(e / (DP / 8), e % (DP / 8))) = qv[i];
       }
       sync();
-      const uint32_t q_base = smem_u32(q_sm);
+      uint32_t q_base = smem_u32(q_sm);
+      pin(q_base);
       const int qrow = (lane & 7) + ((lane >> 3) & 1) * 8;
       uint32_t qa[MT == 1 ? DP / 16 : 1][4];  // one row tile a warp: its fragments stay in registers
       if constexpr (MT == 1) {
@@ -191,7 +196,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
       for (int u = w.tile; u < w.tile + w.count; ++u, ++it) {
         const uint32_t st = it % S::STAGES;
         mbar_wait(&full[st], (it / S::STAGES) & 1, abort_flag, 44);  // on expiry every wait returns: all warps finish
-        const uint32_t k_base = smem_u32(sm + st * 2 * S::TILE), v_base = k_base + S::TILE;
+        uint32_t k_base = smem_u32(sm + st * 2 * S::TILE);
+        pin(k_base);
         // ---- S = Q K^T for the warp's rows and 16 keys
         float s[MT][2][4];
 #pragma unroll
@@ -304,6 +310,8 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             }
           }
         // ---- O += P V
+        uint32_t v_base = k_base + S::TILE;
+        if (open) pin(v_base);  // after the zeros
         if (!poison) {
           const int vrow = kg * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
@@ -342,6 +350,12 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             }
           }
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int nb = 0; nb < DP / 8; ++nb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pin(o[i][nb][j]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }
