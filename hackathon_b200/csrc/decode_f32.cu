@@ -182,7 +182,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int c = 0; c < 3; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
-#pragma unroll 4
+#pragma unroll 2
         for (int ks = 0; ks < DP / 8; ks += 2) {
           uint32_t b[4], bh[4], bl[4];  // two steps of 8 dims
           ldsm4(k_base + at<KEYS>(kg * 8 + (lane & 7), 2 * ks + (lane >> 3)), b);

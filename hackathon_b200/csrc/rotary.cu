@@ -128,6 +128,8 @@ struct Unit {
   int sub, off0, off1;  // the unit's two pieces of VEC elements
   bool active, turned;
   int lanes, own, role; // own: which head of the warp's; role: whose coefficients are held, -1: none
+  static constexpr int SHARE = LANES == 0 ? 1 : 32 / LANES < VEC ? 32 / LANES : VEC;
+  long long steps[LANES ? VEC / SHARE : 1];  // of the pairs the lane works out: pair i * SHARE + g is the warp's head g's
   float c[VEC], s[VEC];
   float ca[VEC], sb[VEC], cb[VEC], sa[VEC];  // pair j: a' = a ca + b sb, b' = b cb + a sa
 
@@ -138,6 +140,10 @@ struct Unit {
     // a piece of each half of the rotated part, or of each half of what is behind it: lanes side by side, pieces too
     off0 = turned ? sub * VEC : a.rotary / 2 + sub * VEC;
     off1 = off0 + (turned ? a.rotary : a.d - a.rotary) / 2;
+    if constexpr (LANES > 0) {
+#pragma unroll
+      for (int i = 0; i < VEC / SHARE; ++i) steps[i] = a.steps[turned ? pair_index(a, i * SHARE + own % SHARE) : 0];
+    }
   }
 
   // The frequency of pair j: (off0 + j, off1 + j), or, interleaved, one of the pairs within the pieces.
@@ -145,16 +151,13 @@ struct Unit {
     return !INTERLEAVED ? sub * VEC + j : j < VEC / 2 ? sub * (VEC / 2) + j : a.rotary / 4 + sub * (VEC / 2) + j - VEC / 2;
   }
 
-  __device__ __forceinline__ void set_token(const Args& a, int b, int t) {
+  __device__ __forceinline__ void set_token(const Args& a, long long pos) {
     role = -1;
-    const long long pos = position(a, b, t);
     if constexpr (LANES > 0) {
-      // pair i * SHARE + g of the unit is worked out by the warp's head g
-      constexpr int SHARE = 32 / LANES < VEC ? 32 / LANES : VEC;
 #pragma unroll
       for (int i = 0; i < VEC / SHARE; ++i) {
         float x, y;
-        turn(pos, a.steps[turned ? pair_index(a, i * SHARE + own % SHARE) : 0], a.scale, x, y);
+        turn(pos, steps[i], a.scale, x, y);
 #pragma unroll
         for (int g = 0; g < SHARE; ++g) {
           c[i * SHARE + g] = __shfl_sync(0xffffffffu, x, sub + g * LANES);
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
   const int first = (item - token * a.chunks) * a.chunk_heads;
   const int last = min(width - (a.copy_v ? 0 : a.heads[2]), first + a.chunk_heads);
   Unit<T, VEC, MODE, INTERLEAVED, 0> unit(a, lane, lanes);
-  unit.set_token(a, b, t);
+  unit.set_token(a, position(a, b, t));
   const int64_t row = cache_row(a, b, t);
   const T* src = static_cast<const T*>(a.in) + (int64_t)token * width * a.d;
   int begin = 0;
@@ -318,6 +321,40 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
         }
       }
     }
+  }
+}
+
+// Tokens of fewer heads than a warp takes at once: heads of several tokens share
+// a warp, each with its own sines.
+template <typename T, int MODE, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) rotary_few_kernel(const Args a, const int lanes, const int64_t items) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  Unit<T, VEC, MODE, INTERLEAVED, 0> unit(a, lane, lanes);
+  const int width = a.heads[0] + a.heads[1] + a.heads[2], total = width - (a.copy_v ? 0 : a.heads[2]);
+  const int64_t item = (((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * (32 / lanes) + unit.own;
+  const bool on = unit.active && item < items;
+  const int token = on ? (int)(item / total) : 0, h = on ? (int)(item - (int64_t)token * total) : 0;
+  const int b = token / a.seq, t = token - b * a.seq;
+  const int role = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+  const int head = h - (role == 0 ? 0 : role == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
+  Piece<T, VEC> p0, p1;
+  if (on) {
+    const T* src = static_cast<const T*>(a.in) + ((int64_t)token * width + h) * a.d;
+    p0.load(src + unit.off0), p1.load(src + unit.off1);
+  }
+  unit.set_token(a, position(a, b, t));
+  int64_t pitch;
+  T* dst = heads_of<T>(a, role, token, b, on ? cache_row(a, b, t) : -1, pitch);
+  const Piece<T, VEC> v0 = p0, v1 = p1;
+  unit.set_role(a, role);
+  unit.head(a, role < 2 ? role : 0, head, on, p0, p1);
+  if (on && dst) {
+    dst += head * pitch;
+    if (role == 2) p0 = v0, p1 = v1;
+    p0.store(dst + unit.off0), p1.store(dst + unit.off1);
   }
 }
 
@@ -383,6 +420,12 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
   for (int i = 0; i < STAGES; ++i) bring(i);
 
   Unit<T, VEC, MODE, INTERLEAVED, LANES> unit(a, lane, LANES);
+  auto position_of = [&](int item) {
+    if (item >= items) return 0ll;
+    const int token = item / a.chunks, b = token / a.seq;
+    return position(a, b, token - b * a.seq);
+  };
+  long long pos = position_of((int)blockIdx.x * WARPS + warp);
   int st = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -390,8 +433,9 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
     const int token = item / a.chunks, first = (item - token * a.chunks) * a.chunk_heads;
     const int last = min(total, first + a.chunk_heads);
     const int b = token / a.seq, t = token - b * a.seq;
-    unit.set_token(a, b, t);
     const int64_t row = cache_row(a, b, t);
+    unit.set_token(a, pos);
+    pos = position_of(item + step);  // of the next item, on its way meanwhile
     for (int h0 = first; h0 < last;) {
       const int n = heads_from(h0, last);
       const int role = h0 < k0 ? 0 : h0 < v0 ? 1 : 2, head = h0 - (role == 0 ? 0 : role == 1 ? k0 : v0);
@@ -490,6 +534,12 @@ static int launch_bulk(const Args& a, int items, cudaStream_t s) {
 template <typename T, int VEC, int MODE, bool INTERLEAVED>
 static int launch(const Args& a, int lanes, int items, cudaStream_t s) {
   if constexpr (VEC * sizeof(T) == 16 && MODE != NORM_EACH) {
+    const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0), hpw = 32 / lanes;
+    if (total < hpw) {
+      const int64_t heads = a.tokens * total;
+      return launch_pdl(rotary_few_kernel<T, MODE, INTERLEAVED>, (int)((heads + 8 * hpw - 1) / (8 * hpw)), 256, 0, s, a, lanes,
+                        heads);
+    }
     switch (lanes) {
       case 4: return launch_bulk<T, MODE, INTERLEAVED, 4>(a, items, s);
       case 8: return launch_bulk<T, MODE, INTERLEAVED, 8>(a, items, s);
