@@ -360,11 +360,11 @@ __global__ void __launch_bounds__(256) rotary_few_kernel(const Args a, const int
 
 // The common case, 16-byte pieces.  HBM bounds it, so the loads need no
 // registers: a warp brings its heads, which lie side by side, into shared memory
-// by bulk copies of up to PIECE bytes of q, k or v heads, STAGES ahead of its
-// work, across tokens.  A warp takes items (a token and chunk_heads of its
-// heads) W apart.
-constexpr int WARPS = 8, STAGES = 3, PIECE = 4096;
-constexpr uint32_t BULK_SMEM = WARPS * STAGES * PIECE;
+// by bulk copies of up to 4 KB of q, k or v heads, as many ahead of its work as
+// fit its 12 KB, across tokens: 12 pieces of up to 1 KB, 6 of 2 KB or 3 of 4 KB.
+// A warp takes items (a token and chunk_heads of its heads) W apart.
+constexpr int WARPS = 8, RING = 12288, MAX_STAGES = 12;
+constexpr uint32_t BULK_SMEM = WARPS * RING;
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -374,17 +374,18 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 template <typename T, int MODE, bool INTERLEAVED, int LANES>
-__global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a, const int items) {
+__global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a, const int items, const int piece) {
   constexpr int VEC = 16 / sizeof(T), HPW = 32 / LANES;
   extern __shared__ __align__(128) uint8_t ring_sm[];
-  __shared__ uint64_t bars[WARPS][STAGES];
+  __shared__ uint64_t bars[WARPS][MAX_STAGES];
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = ring_sm + warp * (STAGES * PIECE);
+  const int stages = RING / piece;
+  uint8_t* ring = ring_sm + warp * RING;
   uint64_t* full = bars[warp];
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[i], 1);
+    for (int i = 0; i < stages; ++i) tc::mbar_init(&full[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::fence_proxy_async();
   }
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int k0 = a.heads[0], v0 = k0 + a.heads[1], width = v0 + a.heads[2], total = a.copy_v ? width : v0;
-  const int per = PIECE / (a.d * (int)sizeof(T)) / HPW * HPW;  // heads of a piece, at most
+  const int per = piece / (a.d * (int)sizeof(T)) / HPW * HPW;  // heads of a piece, at most
   const int step = (int)gridDim.x * WARPS;
   // heads of the piece that begins at head h of a chunk that ends at `last`: all q, all k or all v
   auto heads_from = [&](int h, int last) { return min(per, min(last, h < k0 ? k0 : h < v0 ? v0 : width) - h); };
@@ -412,20 +413,14 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
     if (lane == 0) {
       const uint32_t bytes = (uint32_t)(n * a.d * (int)sizeof(T));
       tc::mbar_arrive_tx(&full[st], bytes);
-      bulk_load(ring + st * PIECE, next_src + next_head * a.d, bytes, &full[st]);
+      bulk_load(ring + st * piece, next_src + next_head * a.d, bytes, &full[st]);
     }
     next_head += n;
     if (next_head >= next_last) next_head = -1, next_item += step;
   };
-  for (int i = 0; i < STAGES; ++i) bring(i);
+  for (int i = 0; i < stages; ++i) bring(i);
 
   Unit<T, VEC, MODE, INTERLEAVED, LANES> unit(a, lane, LANES);
-  auto position_of = [&](int item) {
-    if (item >= items) return 0ll;
-    const int token = item / a.chunks, b = token / a.seq;
-    return position(a, b, token - b * a.seq);
-  };
-  long long pos = position_of((int)blockIdx.x * WARPS + warp);
   int st = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -434,8 +429,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
     const int last = min(total, first + a.chunk_heads);
     const int b = token / a.seq, t = token - b * a.seq;
     const int64_t row = cache_row(a, b, t);
-    unit.set_token(a, pos);
-    pos = position_of(item + step);  // of the next item, on its way meanwhile
+    unit.set_token(a, position(a, b, t));
     for (int h0 = first; h0 < last;) {
       const int n = heads_from(h0, last);
       const int role = h0 < k0 ? 0 : h0 < v0 ? 1 : 2, head = h0 - (role == 0 ? 0 : role == 1 ? k0 : v0);
@@ -449,7 +443,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
       if (dst) {
         unit.set_role(a, role);
         dst += (head + unit.own) * pitch;
-        const T* src = reinterpret_cast<const T*>(ring + st * PIECE) + unit.own * a.d;
+        const T* src = reinterpret_cast<const T*>(ring + st * piece) + unit.own * a.d;
         if (role == 2) {
 #pragma unroll 2
           for (int h = unit.own; h < n; h += HPW, src += HPW * a.d, dst += HPW * pitch) {
@@ -471,7 +465,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
       }
       __syncwarp();  // every lane has read the piece
       bring(st);
-      if (++st == STAGES) st = 0, phase ^= 1;
+      if (++st == stages) st = 0, phase ^= 1;
     }
   }
   if (!ok)  // copies still in flight land before the block's shared memory is given back
@@ -528,14 +522,20 @@ static int launch_bulk(const Args& a, int items, cudaStream_t s) {
   auto kernel = rotary_bulk_kernel<T, MODE, INTERLEAVED, LANES>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_smem(kernel, (int)BULK_SMEM, done)) return rc;
-  return launch_pdl(kernel, blocks < most ? blocks : most, 32 * WARPS, BULK_SMEM, s, a, items);
+  // the largest piece there is: a role's heads, or a chunk's
+  const int heads = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
+  const int64_t bytes = (int64_t)(heads < a.chunk_heads ? heads : a.chunk_heads) * a.d * sizeof(T);
+  const int piece = bytes <= 1024 ? 1024 : bytes <= 2048 ? 2048 : 4096;
+  return launch_pdl(kernel, blocks < most ? blocks : most, 32 * WARPS, BULK_SMEM, s, a, items, piece);
 }
 
 template <typename T, int VEC, int MODE, bool INTERLEAVED>
 static int launch(const Args& a, int lanes, int items, cudaStream_t s) {
   if constexpr (VEC * sizeof(T) == 16 && MODE != NORM_EACH) {
     const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0), hpw = 32 / lanes;
-    if (total < hpw) {
+    // sines for each head cost more than they save from one and a half rounds on: 5 heads of 96 11.6 us against 18,
+    // 4 of 128 25.5 against 28.8, but 12 of 64 (eight a round) 37 against 32
+    if (2 * total < 3 * hpw) {
       const int64_t heads = a.tokens * total;
       return launch_pdl(rotary_few_kernel<T, MODE, INTERLEAVED>, (int)((heads + 8 * hpw - 1) / (8 * hpw)), 256, 0, s, a, lanes,
                         heads);
