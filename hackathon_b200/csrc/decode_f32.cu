@@ -45,10 +45,15 @@ __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x) : : "m
 
 // x = hi + lo for tf32 products, which ignore the low 13 bits: hi is x rounded to
 // the 11 that count, lo the rest, of which they see 11 more.  Where x is infinite
-// hi alone carries it.
+// hi alone carries it, and `part`, hi for the products with another value's lo
+// (which may be 0 or of the other sign), is 0.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = fabsf(x) == INFINITY ? 0u : __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo, uint32_t& part) {
+  split(x, hi, lo);
+  part = fabsf(x) == INFINITY ? 0u : hi;
 }
 
 // Byte offset of 16-byte chunk `ch` (4 dims) of row `row` in a tile of 128-byte
@@ -184,10 +189,10 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
           for (int c = 0; c < 3; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
 #pragma unroll 2
         for (int ks = 0; ks < DP / 8; ks += 2) {
-          uint32_t b[4], bh[4], bl[4];  // two steps of 8 dims
+          uint32_t b[4], bh[4], bl[4], bp[4];  // two steps of 8 dims
           ldsm4(k_base + at<KEYS>(kg * 8 + (lane & 7), 2 * ks + (lane >> 3)), b);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) split(__uint_as_float(b[c]), bh[c], bl[c]);
+          for (int c = 0; c < 4; ++c) split(__uint_as_float(b[c]), bh[c], bl[c], bp[c]);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
               ldsm4(q_at + S::ROWS * DP * 4, fl);
               mma(acc[i][0], fh, bh[2 * h], bh[2 * h + 1]);
               mma(acc[i][1], fh, bl[2 * h], bl[2 * h + 1]);
-              mma(acc[i][2], fl, bh[2 * h], bh[2 * h + 1]);
+              mma(acc[i][2], fl, bp[2 * h], bp[2 * h + 1]);
             }
         }
 #pragma unroll
@@ -287,12 +292,12 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
 #pragma unroll
           for (int nb = 0; nb < DP / 8; ++nb) {
             const int ch = 2 * nb + (g >> 2);
-            uint32_t h0, l0, h1, l1;
-            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r, ch) + 4 * (g & 3)), h0, l0);
-            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r + 1, ch) + 4 * (g & 3)), h1, l1);
+            uint32_t h0, l0, p0, h1, l1, p1;
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r, ch) + 4 * (g & 3)), h0, l0, p0);
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r + 1, ch) + 4 * (g & 3)), h1, l1, p1);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-              mma(o[i][nb], pl[i], h0, h1);
+              mma(o[i][nb], pl[i], p0, p1);
               mma(o[i][nb], ph[i], l0, l1);
               mma(o[i][nb], ph[i], h0, h1);
             }

@@ -631,8 +631,11 @@ int launch_rotary(const c3b_tensor* in, const c3b_tensor& out, const c3b_rotary_
   C3B_REQUIRE(is_float(x.dtype) && out.dtype == x.dtype, "rotary: f32, bf16 or fp16, the same in and out");
   C3B_REQUIRE(x.ndim == 4, "rotary: x is [batch, tokens, heads, head_dim]");
   C3B_REQUIRE(numel(out) == numel(x), "rotary: the output is shaped like x");
-  C3B_REQUIRE(x.shape[1] < (1ll << 31) && x.shape[2] < (1 << 24) && x.shape[3] <= 65536, "rotary: extents too large");
-  C3B_REQUIRE(x.ptr == out.ptr || !overlaps(x, out), "rotary: x and the output are the same buffer or do not overlap");
+  C3B_REQUIRE(x.shape[1] < (1ll << 31) && x.shape[2] < (1 << 24) && x.shape[3] <= 65536 &&
+                  x.shape[2] * x.shape[3] < (1ll << 31),
+              "rotary: extents too large");
+  C3B_REQUIRE((x.ptr == out.ptr || !overlaps(x, out)) && !overlaps(pos, out) && !overlaps(steps, out),
+              "rotary: x and the output are the same buffer or do not overlap, nor does another input");
   Args a = {};
   a.in = x.ptr;
   a.out[0] = out.ptr;
@@ -659,13 +662,17 @@ int launch_qk_norm_rotary(const c3b_tensor* in, int n_in, const c3b_tensor* out,
   const c3b_tensor &pos = in[1 + n_w], &steps = in[2 + n_w];
   C3B_REQUIRE(p.batch >= 0 && p.seq >= 0 && p.heads >= 0 && p.kv_heads >= 0 && p.head_dim > 0 && p.head_dim <= 65536,
               w + ": bad extents");
-  C3B_REQUIRE(p.seq < (1ll << 31) && p.heads < (1 << 24) && p.kv_heads < (1 << 24), w + ": extents too large");
   const int64_t width = p.heads + 2ll * p.kv_heads;
+  C3B_REQUIRE(p.seq < (1ll << 31) && p.heads < (1 << 24) && p.kv_heads < (1 << 24) && width * p.head_dim < (1ll << 31),
+              w + ": extents too large");
   C3B_REQUIRE(is_float(x.dtype), w + ": f32, bf16 or fp16");
   C3B_REQUIRE(numel(x) == p.batch * p.seq * width * p.head_dim, w + ": qkv is [batch, tokens, heads + 2 kv_heads, head_dim]");
   C3B_REQUIRE(std::isfinite(p.scale) && p.epsilon >= 0.f, w + ": the scale is finite, epsilon at least 0");
   C3B_REQUIRE(p.normalize || n_w == 0, w + ": weights without normalisation");
-  for (int i = 0; i < n_out; ++i) C3B_REQUIRE(out[i].dtype == x.dtype, w + ": outputs have the type of qkv");
+  for (int i = 0; i < n_out; ++i) {
+    C3B_REQUIRE(out[i].dtype == x.dtype, w + ": outputs have the type of qkv");
+    for (int j = 1; j < n_in; ++j) C3B_REQUIRE(!overlaps(out[i], in[j]), w + ": an output overlaps an input");
+  }
   Args a = {};
   a.in = x.ptr;
   a.tokens = p.batch * p.seq;

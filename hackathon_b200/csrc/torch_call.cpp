@@ -166,10 +166,17 @@ PyObject* state_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
       PyErr_Format(PyExc_RuntimeError, "%s failed (%d): %s", s->name->c_str(), rc, g_error());
       return nullptr;
     }
-    for (const auto& v : r.shapes) {
-      PyObject* view = PyObject_CallMethod(PyList_GET_ITEM(args[1], v.first), "view", "O", v.second);
-      if (!view || PyList_SetItem(args[1], v.first, view) < 0) return nullptr;
+    if (r.shapes.empty()) Py_RETURN_NONE;
+    // `view` is Python's: hold the shapes, since what it runs may make calls of its own
+    std::vector<std::pair<Py_ssize_t, PyObject*>> shapes(r.shapes);
+    for (auto& v : shapes) Py_INCREF(v.second);
+    bool ok = true;
+    for (auto& v : shapes) {
+      PyObject* view = ok ? PyObject_CallMethod(PyList_GET_ITEM(args[1], v.first), "view", "O", v.second) : nullptr;
+      ok = ok && view && PyList_SetItem(args[1], v.first, view) == 0;
+      Py_DECREF(v.second);
     }
+    if (!ok) return nullptr;
     Py_RETURN_NONE;
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());

@@ -87,6 +87,8 @@ def describe(x: Any) -> Desc:
             raise ValueError("kernel arrays must be C-contiguous")
         dmap = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16, torch.int64: L.I64,
                 torch.int32: L.I32, torch.uint8: L.U8, torch.bool: L.U8}
+        if x.dtype not in dmap:
+            raise TypeError(f"unsupported dtype {x.dtype}")
         return Desc(int(x.data_ptr()), dmap[x.dtype], tuple(int(d) for d in x.shape))
     cai = getattr(x, "__cuda_array_interface__", None)
     if cai is None:

@@ -171,6 +171,11 @@ REFUSED = {
     "rotary: steps as floats": rotary_call(steps=lambda n: n(L.F32, D // 2)),
     "rotary: output half over the input": rotary_call(x=Desc(1 << 20, L.BF16, (B, S, HQ, D)),
                                                       out=Desc((1 << 20) + 128, L.BF16, (B, S, HQ, D))),
+    "rotary: output over the positions": rotary_call(pos=Desc(1 << 30, L.I64, (B, S)), out=Desc(1 << 30, L.BF16, (B, S, HQ, D))),
+    "rotary: a token of more than 2**31 elements": rotary_call(x=lambda n: n(L.BF16, 1, 1, 1 << 23, 256), pos=lambda n: n(L.I64, 1, 1),
+                                                               out=lambda n: n(L.BF16, 1, 1, 1 << 23, 256)),
+    "norm: output over a weight": norm_call(qw=Desc(1 << 30, L.F32, (D,)), out=Desc(1 << 30, L.F16, (B, S, HQ + 2 * HK, D))),
+    "append: cache over the lengths": append_call(lengths=Desc(1 << 30, L.I32, (B,)), k=Desc(1 << 30, L.F32, (B, HK, C, D))),
     "norm: heads do not add up": norm_call({"kv_num_heads": 1}),
     "norm: weights without normalisation": norm_call({"normalize": 0}),
     "norm: weight of another size": norm_call(qw=lambda n: n(L.F32, D // 2)),
@@ -198,6 +203,9 @@ REFUSED = {
     "tree: output of another type": tree_call(out=lambda n: n(L.F32, B, S, HQ, D)),
     "tree: scale is no number": tree_call({"scale": float("nan")}),
     "tree: negative scale": tree_call({"scale": -0.125}),
+    "tree: no workspace": tree_call(k=lambda n: n(L.BF16, B, HK, 600, D), v=lambda n: n(L.BF16, B, HK, 600, D)),
+    "tree: workspace too small": (lambda c: (c[0], c[1], c[2] + [Desc(1 << 30, L.U8, (1000,))], c[3]))(
+        tree_call(k=lambda n: n(L.BF16, B, HK, 600, D), v=lambda n: n(L.BF16, B, HK, 600, D))),
     "commit: path int64": commit_call(path=lambda n: n(L.I64, B, 3)),
     "commit: path rank": commit_call(path=lambda n: n(L.I32, B)),
     "commit: accepted of another size": commit_call(acc=lambda n: n(L.I32, B + 1)),

@@ -566,3 +566,107 @@ def test_in_a_native_plan(t):
     call("qk_norm_rotary_append", [qkv, None, None, t.tensor(pos).cuda(), t.tensor(steps).cuda(), d_len], [q, kc, vc], {"num_heads": H})
     o = call("tree_attention", [q, kc, vc, d_len], [t.empty_like(q)])[0]
     assert np.array_equal(bits(o), got)
+
+
+def test_in_a_native_plan_with_a_workspace(t):
+    """A cache long enough to be split: the plan's arena holds the workspace; two replays of its graph agree with the
+    eager call."""
+    from hackathon_b200 import _lib as L
+    from hackathon_b200 import kernels as K
+    from hackathon_b200.runtime import NativePlan
+    B, T, HQ, HK, D, C = 2, 5, 8, 2, 128, 3000
+    q, k, v, lengths, mask = tree_inputs(t, (T, HQ, HK, D, C, [2990, 411]), "bf16")
+    bits = lambda x: x.view(t.int16).cpu().numpy()  # noqa: E731
+    ws = K.tree_attention_workspace(K.Desc(0, L.BF16, (B, T, HQ, D)), K.Desc(0, L.BF16, (B, HK, C, D)))
+    assert ws > 0
+    host_of = dict(q=bits(q), k=bits(k), v=bits(v), lengths=lengths.cpu().numpy(), mask=mask.astype(np.uint8),
+                   o=np.zeros((B, T, HQ, D), np.int16), ws=np.full(ws, 255, np.uint8))
+    offs, at = {}, 0
+    for name, arr in host_of.items():
+        offs[name] = at
+        at += (arr.nbytes + 255) // 256 * 256
+    plan = NativePlan(at, 1, 0)
+    try:
+        for name, arr in host_of.items():
+            plan.upload(offs[name], np.ascontiguousarray(arr))
+        d = lambda name, dt, *shape: K.Desc(offs[name], dt, shape, arena=True)  # noqa: E731
+        ln, = K.prepare("tree_attention", [d("q", L.BF16, B, T, HQ, D), d("k", L.BF16, B, HK, C, D), d("v", L.BF16, B, HK, C, D),
+                                           d("lengths", L.I32, B), d("mask", L.U8, B, T, T)],
+                        [d("o", L.BF16, B, T, HQ, D), d("ws", L.U8, ws)], {}).launches
+        plan.kernel(0, ln)
+        plan.finalize(True)
+        want = bits(call("tree_attention", [q, k, v, lengths, t.tensor(mask).cuda()], [t.empty_like(q)])[0])
+        for _ in range(2):
+            plan.run()
+            assert np.array_equal(plan.download(offs["o"], np.zeros((B, T, HQ, D), np.int16)), want)
+    finally:
+        plan.close()
+
+
+def test_general_path_matches_the_native_binding(t):
+    """What serves arrays of other libraries, with torch's as the scratch: the same bits."""
+    from hackathon_b200 import kernel_registry as R
+    q, k, v, lengths, mask = tree_inputs(t, (5, 8, 2, 128, 3000, [2990, 411]), "bf16")
+    want = call("tree_attention", [q, k, v, lengths, None], [t.empty_like(q)])[0]
+    outs = [t.empty(q.numel(), dtype=q.dtype, device="cuda")]  # flat: comes back in its logical shape
+    R._with_workspace(R._make("tree_attention"), "tree_attention", [q, k, v, lengths, None], outs, {})
+    t.cuda.synchronize()
+    assert len(outs) == 1 and t.equal(outs[0], want)
+    outs = call("tree_attention", [q, k, v, lengths, None], [t.empty(q.numel(), dtype=q.dtype, device="cuda")])
+    assert outs[0].shape == q.shape and t.equal(outs[0], want)
+
+
+def test_two_streams_at_once(t):
+    """Calls that overlap on the GPU have workspaces of their own."""
+    sets = [tree_inputs(t, (9, 16, 2, 128, 20000, [19991, 7000, 13]), "bf16", seed=60 + i) for i in range(2)]
+    want = [call("tree_attention", [q, k, v, n, t.tensor(m).cuda()], [t.empty_like(q)])[0] for q, k, v, n, m in sets]
+    masks = [t.tensor(s[4]).cuda() for s in sets]
+    t.cuda.synchronize()
+    streams = [t.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with t.cuda.stream(s):
+                q, k, v, n, _ = sets[i]
+                got[i].append(call_async("tree_attention", [q, k, v, n, masks[i]], [t.empty_like(q)])[0])
+    t.cuda.synchronize()
+    for i in range(2):
+        assert all(t.equal(x, want[i]) for x in got[i])
+
+
+def call_async(name, ins, outs, params=None):
+    from hackathon_b200.kernel_registry import lookup
+    lookup(name)(ins, outs, params or {})
+    return outs
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("d,hq", [(64, 2), (64, 12), (128, 4), (128, 40), (96, 24), (256, 2), (17, 2)])
+def test_committed_poison_reaches_the_rows_that_see_it(t, d, hq, dtype):
+    """A NaN key makes every row of its sequence and kv head NaN; an infinite value makes its dim infinite; another
+    sequence and head are as they were."""
+    T, hk, cap = 3, 2, 400
+    q, k, v, lengths, mask = tree_inputs(t, (T, hq, hk, d, cap, [390, 390, 390]), dtype)
+    clean = call("tree_attention", [q, k, v, lengths, t.tensor(mask).cuda()], [t.empty_like(q)])[0]
+    k[0, 0, 100] = float("nan")
+    v[1, 1, 77, 3] = float("inf")
+    out = call("tree_attention", [q, k, v, lengths, t.tensor(mask).cuda()], [t.empty_like(q)])[0]
+    g = hq // hk
+    assert t.isnan(out[0, :, :g]).all()
+    assert t.isposinf(out[1, :, g:, 3]).all()
+    keep = t.ones_like(out, dtype=t.bool)
+    keep[0, :, :g] = False
+    keep[1, :, g:, 3] = False
+    assert t.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_sequences_and_ragged_lengths(t, dtype):
+    """More sequences than a warp has lanes, most of them empty or short, beside one that is long."""
+    lengths = [0, 1, 63, 64, 65, 127, 128, 129] * 9 + [2900, 0, 5]
+    case = (2, 4, 2, 64, 2999, lengths)
+    q, k, v, n, mask = tree_inputs(t, case, dtype)
+    out = call("tree_attention", [q, k, v, n, t.tensor(mask).cuda()], [t.full_like(q, 7.0)])[0]
+    want, size, ulps = O.tree_attention(host(q), host(k), host(v), lengths, mask, 0.125)
+    close(out, want, tree_tolerance(want, size, ulps, dtype))
+    assert status() == 0
