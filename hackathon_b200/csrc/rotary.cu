@@ -174,6 +174,17 @@ struct Unit {
     }
   }
 
+  // The same from a token's cosines and sines, worked out before.
+  __device__ __forceinline__ void take_token(const Args& a, const float* cosines, const float* sines) {
+    role = -1;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int p = turned ? pair_index(a, j) : 0;
+      c[j] = turned ? cosines[p] : 1.f;
+      s[j] = turned ? sines[p] : 0.f;
+    }
+  }
+
   __device__ __forceinline__ void set_role(const Args& a, int r) {
     if (r == role || r == 2) return;
     role = r;
@@ -324,19 +335,33 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
   }
 }
 
-// Tokens of fewer heads than a warp takes at once: heads of several tokens share
-// a warp, each with its own sines.
-template <typename T, int MODE, bool INTERLEAVED>
+// Tokens of few heads: heads of several tokens share a warp.  SHARED: the block
+// first works out the sines of its tokens, each once, into shared memory; else
+// each lane those of its pairs.
+template <typename T, int MODE, bool INTERLEAVED, bool SHARED>
 __global__ void __launch_bounds__(256) rotary_few_kernel(const Args a, const int lanes, const int64_t items) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int VEC = 16 / sizeof(T);
+  constexpr int MOST = SHARED ? 256 * VEC / 3 : 0;  // pairs of a block's tokens
+  __shared__ __align__(16) float cosines[MOST + 1], sines[MOST + 1];
+  __shared__ long long positions[SHARED ? 64 : 1];  // a block takes at most 8 * 32 / 4 heads
   const int lane = threadIdx.x & 31;
   Unit<T, VEC, MODE, INTERLEAVED, 0> unit(a, lane, lanes);
   const int width = a.heads[0] + a.heads[1] + a.heads[2], total = width - (a.copy_v ? 0 : a.heads[2]);
-  const int64_t item = (((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * (32 / lanes) + unit.own;
-  const bool on = unit.active && item < items;
-  const int token = on ? (int)(item / total) : 0, h = on ? (int)(item - (int64_t)token * total) : 0;
+  const int per_block = 8 * (32 / lanes), half = a.rotary / 2, item = (threadIdx.x >> 5) * (32 / lanes) + unit.own;
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  const bool on = unit.active && first + item < items;
+  int token0 = 0, tokens = 0, token, h;
+  if constexpr (SHARED) {  // the block's heads: of tokens token0 .. token0 + tokens - 1, from head h0 of the first
+    token0 = items >> 31 ? (int)(first / total) : (int)((uint32_t)first / (uint32_t)total);
+    const int h0 = (int)(first - (int64_t)token0 * total), here = items - first < per_block ? (int)(items - first) : per_block;
+    tokens = (h0 + here - 1) / total + 1;
+    const int nth = (h0 + item) / total;
+    token = on ? token0 + nth : token0, h = on ? h0 + item - nth * total : 0;
+  } else {
+    token = on ? (int)((first + item) / total) : 0, h = on ? (int)(first + item - (int64_t)token * total) : 0;
+  }
   const int b = token / a.seq, t = token - b * a.seq;
   const int role = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
   const int head = h - (role == 0 ? 0 : role == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
@@ -345,9 +370,28 @@ __global__ void __launch_bounds__(256) rotary_few_kernel(const Args a, const int
     const T* src = static_cast<const T*>(a.in) + ((int64_t)token * width + h) * a.d;
     p0.load(src + unit.off0), p1.load(src + unit.off1);
   }
-  unit.set_token(a, position(a, b, t));
+  if (SHARED) {
+    if (threadIdx.x < tokens) {
+      const int tk = token0 + threadIdx.x, bb = tk / a.seq;
+      positions[threadIdx.x] = position(a, bb, tk - bb * a.seq);
+    }
+    int p = threadIdx.x % half, i = threadIdx.x / half;
+    const int dp = 256 % half, di = 256 / half;
+    __syncthreads();
+    for (; i < tokens; p += dp, i += di) {
+      if (p >= half && ++i >= tokens) break;
+      if (p >= half) p -= half;
+      turn(positions[i], a.steps[p], a.scale, cosines[i * half + p], sines[i * half + p]);
+    }
+  }
   int64_t pitch;
   T* dst = heads_of<T>(a, role, token, b, on ? cache_row(a, b, t) : -1, pitch);
+  if (SHARED) {
+    __syncthreads();
+    unit.take_token(a, cosines + (token - token0) * half, sines + (token - token0) * half);
+  } else {
+    unit.set_token(a, position(a, b, t));
+  }
   const Piece<T, VEC> v0 = p0, v1 = p1;
   unit.set_role(a, role);
   unit.head(a, role < 2 ? role : 0, head, on, p0, p1);
@@ -533,12 +577,17 @@ template <typename T, int VEC, int MODE, bool INTERLEAVED>
 static int launch(const Args& a, int lanes, int items, cudaStream_t s) {
   if constexpr (VEC * sizeof(T) == 16 && MODE != NORM_EACH) {
     const int total = a.heads[0] + a.heads[1] + (a.copy_v ? a.heads[2] : 0), hpw = 32 / lanes;
-    // sines for each head cost more than they save from one and a half rounds on: 5 heads of 96 11.6 us against 18,
-    // 4 of 128 25.5 against 28.8, but 12 of 64 (eight a round) 37 against 32
-    if (2 * total < 3 * hpw) {
+    // 12 heads of 64 (eight a round) 30 us against 35, 5 of 96 11 against 18; from two rounds on the bulk copies win:
+    // 8 heads of 128 38 us against 41, 24 of 64 42 against 55
+    if (total < 2 * hpw) {
       const int64_t heads = a.tokens * total;
-      return launch_pdl(rotary_few_kernel<T, MODE, INTERLEAVED>, (int)((heads + 8 * hpw - 1) / (8 * hpw)), 256, 0, s, a, lanes,
-                        heads);
+      const int per_block = 8 * hpw, blocks = (int)((heads + per_block - 1) / per_block);
+      // Sines worked out once for a block cost as much as two and a half times as many of a lane's own:
+      // 4 heads of 64 45 us against 48, 3 heads 48 either way, 2 heads 54 against 48.
+      const int most = total == 1 ? per_block : (per_block - 2) / total + 2;  // tokens that a block's heads touch
+      const bool shared = 3 * most * (a.rotary / 2) <= 256 * VEC;
+      return launch_pdl(shared ? rotary_few_kernel<T, MODE, INTERLEAVED, true> : rotary_few_kernel<T, MODE, INTERLEAVED, false>,
+                        blocks, 256, 0, s, a, lanes, heads);
     }
     switch (lanes) {
       case 4: return launch_bulk<T, MODE, INTERLEAVED, 4>(a, items, s);

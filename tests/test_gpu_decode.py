@@ -101,6 +101,23 @@ def test_rotary(t, case, interleaved, dtype):
     assert t.equal(outs2[0], outs[0])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,r", [(64, 64), (64, 16), (96, 48), (128, 128), (256, 128)])
+@pytest.mark.parametrize("heads", [1, 2, 3, 4, 5, 7, 9, 13, 15])
+def test_rotary_of_few_heads(t, heads, d, r, dtype):
+    """Blocks whose heads begin and end within a token, and whose tokens are of several sequences."""
+    for interleaved, (b, s) in enumerate([(13, 29), (5, 1)]):
+        x = values(t, dtype, b, s, heads, d, seed=heads)
+        steps = rotary.rotary_steps(r, 10000.0)[0]
+        pos = np.random.default_rng(heads).integers(0, 1 << 20, (b, s))
+        out = call("rotary_embedding", [x, t.tensor(pos).cuda(), t.tensor(steps).cuda()], [t.empty_like(x)],
+                   {"interleaved": interleaved, "scale": 0.75})[0]
+        want = O.turned(host(x), pos, steps, 0.75, interleaved)
+        tol = 2.0 ** -20 * O.pair_size(host(x), r, 0.75, interleaved) + HALF_STEP[dtype] * np.abs(want) + 1e-7
+        tol[..., r:] = 0
+        close(out, want, tol)
+
+
 def test_rotary_positions(t):
     """Shared, 32-bit, negative and very far positions; a zero position leaves x as it is."""
     x = values(t, "f32", 3, 4, 2, 64, seed=4)
@@ -204,7 +221,8 @@ def test_qk_norm_of_zero_and_small_heads(t):
 APPEND = [  # case as above, capacity, lengths
     ((2, 1, 4, 4, 64, 64, 0, 0), 9, [0, 8]), ((3, 5, 32, 8, 128, 128, 1, 0), 40, [0, 17, 35]),
     ((2, 7, 3, 1, 80, 20, 0, 0), 7, [0, 0]), ((1, 63, 2, 2, 64, 32, 0, 0), 1000, [501]),
-    ((2, 3, 4, 2, 50, 10, 1, 1), 11, [3, 8]),
+    ((2, 3, 4, 2, 50, 10, 1, 1), 11, [3, 8]), ((3, 21, 2, 1, 64, 64, 0, 0), 60, [0, 11, 39]),
+    ((5, 9, 2, 2, 64, 64, 0, 0), 20, [0, 1, 11, 3, 7]),
 ]
 
 
