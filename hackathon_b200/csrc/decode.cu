@@ -296,7 +296,8 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
               "tree attention: heads is a multiple of kv_heads");
   C3B_REQUIRE(p.head_dim >= 1 && p.head_dim <= 256, "tree attention: head_dim is 1 to 256");
   C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), "tree attention: bad capacity");
-  C3B_REQUIRE(std::isfinite(p.scale) && p.scale > 0.f, "tree attention: the scale is positive");
+  // the kernels multiply by scale / ln 2
+  C3B_REQUIRE(std::isfinite(p.scale * 1.4426950408889634f) && p.scale > 0.f, "tree attention: the scale is positive and below 2e38");
   const int64_t rows = (int64_t)p.batch * p.tokens * p.heads;
   C3B_REQUIRE(numel(q) == rows * p.head_dim && numel(out[0]) == numel(q),
               "tree attention: q and the output are [batch, tokens, heads, head_dim]");

@@ -351,7 +351,7 @@ typedef struct {
 } c3b_qk_norm_params;
 
 /* --- C3B_K_TREE_ATTN: inputs q [B, T, heads, D], k cache, v cache, lengths,
- * [mask]; output [B, T, heads, D] = softmax(q k^T scale) v, scale > 0.  Draft i of a
+ * [mask]; output [B, T, heads, D] = softmax(q k^T scale) v, 0 < scale < 2e38.  Draft i of a
  * sequence sees its committed rows and the drafts j with mask[i][j] != 0 (one
  * byte each): mask_mode 0 none given, a chain (j <= i); 1 [T, T] for all
  * sequences; 2 [B, T, T].  A row that sees nothing is zero.  Head h reads kv
