@@ -21,7 +21,10 @@
 //
 // Values behind the drafts are zeroed in shared memory before they are
 // multiplied; so are drafts' values that hold infinities or NaN, and those are
-// then added row by row where the mask lets them through.
+// then added row by row where the mask lets them through.  Where both groups
+// read the same unit, group 0 alone does that: the issuing thread waits for
+// group 0's weights of a unit before it goes on to group 1's, so group 1's
+// product finds the unit cleared as well.
 #include <type_traits>
 
 #include "common.cuh"
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         const int key0 = (w.tile + k) * KEYS;
         const bool open = key0 + KEYS > w.n;  // the unit reaches past the committed rows
-        if (open) {
+        if (open && !(two && grp)) {
           // values behind the drafts, and drafts' that are not finite, become zero: one key a thread
           const uint32_t ld = base + 2 * k + 1, st = ld % S::SLOTS;
           mbar_wait(&full[st], (ld / S::SLOTS) & 1, abort_flag, 47);
