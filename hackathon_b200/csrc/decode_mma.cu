@@ -266,6 +266,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             }
           }
           fence_proxy_async();  // these writes come before the next load into the stage
+          __syncwarp();         // and before the other lanes read the unit
           poison = __any_sync(0xffffffffu, poison);
         }
         // ---- running maxima

@@ -50,3 +50,20 @@ def test_infinite_drafts_count_once(t, T, hq, hk, d, dtype):
     tol = tree_tolerance(want, size, ulps, dtype) + POLYNOMIAL * size
     close(out[..., t.tensor(rest).cuda()], want[..., rest], tol[..., rest])
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("T,hq,d,cap", [(1, 4, 64, 100), (3, 12, 128, 400), (2, 40, 64, 400), (1, 24, 256, 300), (4, 64, 128, 300)])
+def test_stale_rows_at_every_offset(t, T, hq, d, cap, dtype):
+    """Whatever stands behind the drafts, at each of a unit's rows: the bits of a call with zeros there."""
+    lengths = list(range(0, 96, 2)) + list(range(97, 97 - 32, -2))
+    q, k, v, n, mask = tree_inputs(t, (T, hq, 2, d, cap, lengths), dtype, seed=71)
+    d_mask = t.tensor(mask).cuda()
+    behind = (t.arange(cap).cuda() >= n[:, None] + T)[:, None, :, None]
+    want = call("tree_attention", [q, k.masked_fill(behind, 0), v.masked_fill(behind, 0), n, d_mask], [t.empty_like(q)])[0]
+    assert t.isfinite(want).all()
+    for fill in (float("nan"), float("inf")):
+        kk, vv = k.masked_fill(behind, fill), v.masked_fill(behind, fill)
+        for _ in range(5):
+            assert t.equal(call("tree_attention", [q, kk, vv, n, d_mask], [t.empty_like(q)])[0], want)
+    assert status() == 0
