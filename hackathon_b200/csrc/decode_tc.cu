@@ -362,9 +362,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           top *= a.scale_log2;
           if (!(top < INFINITY)) l = NAN;  // a NaN or an infinite score: so is the row, as its definition has it
-          const bool grow = top > m + 8.0f;
+          const bool grow = top > m + (dec::LAG + dec::lift(H16));  // m: the reference of dec::LAG and dec::lift
           if (__any_sync(0xffffffffu, grow)) {
-            const float mn = grow ? fmaxf(m, top) : m;
+            const float mn = grow ? top - dec::lift(H16) : m;
             const float f = mn == -INFINITY ? 1.f : exp2_sfu(m - mn);
             l *= f;
             m = mn;

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from oracle import decode as O
-from test_gpu_decode import HALF_STEP, U, call, close, host, status, tree_inputs, tree_tolerance
+from test_gpu_decode import HALF_STEP, U, call, close, host, status, tree_inputs, tree_tolerance, values
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,39 @@ def test_stale_rows_at_every_offset(t, T, hq, d, cap, dtype):
         for _ in range(5):
             assert t.equal(call("tree_attention", [q, kk, vv, n, d_mask], [t.empty_like(q)])[0], want)
     assert status() == 0
+
+
+SHAPES = [(1, 4, 1), (5, 4, 1), (10, 8, 1), (40, 8, 1)]  # tokens, q heads, kv heads: 4, 20, 80, 320 rows of a kv head
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("nats", [9, 14, 16, 17])
+@pytest.mark.parametrize("cap", [256, 1000])
+@pytest.mark.parametrize("T,hq,hk", SHAPES)
+def test_tail_far_below_the_largest_scores(t, T, hq, hk, cap, nats, dtype):
+    """Every other key `nats` above the rest, with values of 0: tiny weights, alike, on values with a mean are the
+    whole output.
+
+    fp16 weights are at least 2**7 where the largest stands, so a weight is off by half a step of its own or, below
+    fp16's normal range, by 2**-25: 2**-32 of the largest."""
+    n, d = cap - T, 64
+    q, k, v = (values(t, dtype, *s, seed=80 + i) for i, s in enumerate([(1, T, hq, d), (1, hk, cap, d), (1, hk, cap, d)]))
+    q.zero_()
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[:, :, ::2, 0] = nats                     # 8 * nats / sqrt(64)
+    v.mul_(0.25).add_(1.0).mul_(2.0 ** 13)
+    v[:, :, ::2] = 0.0
+    out = call("tree_attention", [q, k, v, t.tensor([n], dtype=t.int32).cuda(), None], [t.empty_like(q)])[0]
+    vv = v[0, 0].double()
+    for tok in range(T):
+        rows = n + tok + 1
+        total = (rows + 1) // 2 * np.exp(float(nats)) + rows // 2
+        want = host(vv[:rows].sum(0) / total)
+        size = host(vv[:rows].abs().sum(0) / total)
+        ulps = 8 * nats + rows + 16            # scores: products of whole numbers, the scale, the base-2 argument; the sums
+        half = HALF_STEP[dtype]
+        tol = (2 * ulps * U + (0 if dtype == "f32" else half) + POLYNOMIAL) * size + half * np.abs(want)
+        if dtype == "fp16":
+            tol = tol + rows * 2.0 ** -32 * np.exp(float(nats)) / total * host(vv[:rows].abs().amax(0))
+        close(out[0, tok], np.broadcast_to(want, (hq, d)), tol)
