@@ -36,10 +36,11 @@ struct Args {
 // which skips most rescales of the sums.  fp16 weights are lifted as far as the
 // type reaches (2^(LAG + lift) = 2^15): they lose bits only below 2^-21 of the
 // largest weight, and none above 2^-32 of it is lost.  bf16 and fp32 have
-// exponents to spare.  The factor is the same in sums of weights and of weighted
-// values, and drops out of their quotient.
+// exponents to spare, but so do their values: their weights are at most 1, so
+// that a weighted value stays within the type.  The factor is the same in sums
+// of weights and of weighted values, and drops out of their quotient.
 constexpr float LAG = 8.f;
-__host__ __device__ constexpr float lift(bool h16) { return h16 ? 7.f : 0.f; }
+__host__ __device__ constexpr float lift(bool h16) { return h16 ? 7.f : -LAG; }
 
 // How a call runs (host).
 struct Plan {

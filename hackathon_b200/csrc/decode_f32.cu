@@ -243,7 +243,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
           __syncwarp();         // and before the other lanes read the unit
           poison = __any_sync(0xffffffffu, poison);
         }
-        // ---- running maxima
+        // ---- running maxima; m is the reference of dec::LAG and dec::lift
         bool grow = false;
         float top[MT][2];
 #pragma unroll
@@ -254,14 +254,14 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             top[i][half] = x;
-            grow = grow || x > m[i][half] + 8.0f;
+            grow = grow || x > m[i][half] + (dec::LAG + dec::lift(false));
           }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const float mn = fmaxf(m[i][half], top[i][half]);
+              const float mn = fmaxf(m[i][half], top[i][half] - dec::lift(false));
               const float f = mn == -INFINITY ? 1.f : exp2f(m[i][half] - mn);
               m[i][half] = mn;
               l[i][half] *= f;

@@ -189,14 +189,14 @@ __global__ void __launch_bounds__((Shape<DP, RW>::THREADS), 1)
           for (int pass = 0; pass < S::PASSES; ++pass)
             if (!dec::visible(a, w, tok, key0 + pass * S::KPP + kk)) s[pass] = -INFINITY;
         }
-        // ---- the row's running maximum, raised lazily; all lanes of a row agree
+        // ---- the row's running maximum, raised lazily; all lanes of a row agree; m is the reference of dec::LAG, dec::lift
         float top = s[0];
 #pragma unroll
         for (int pass = 1; pass < S::PASSES; ++pass) top = fmaxf(top, s[pass]);
 #pragma unroll
         for (int x = S::LK; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-          const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : exp2f(m - mn);
+        if (__any_sync(0xffffffffu, top > m + (dec::LAG + dec::lift(false)))) {
+          const float mn = fmaxf(m, top - dec::lift(false)), f = mn == -INFINITY ? 1.f : exp2f(m - mn);
           m = mn;
           l *= f;
 #pragma unroll

@@ -103,3 +103,26 @@ def test_tail_far_below_the_largest_scores(t, T, hq, hk, cap, nats, dtype):
         if dtype == "fp16":
             tol = tol + rows * 2.0 ** -32 * np.exp(float(nats)) / total * host(vv[:rows].abs().amax(0))
         close(out[0, tok], np.broadcast_to(want, (hq, d)), tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,hq,hk,d", [(1, 1, 1, 64), (1, 4, 1, 128), (2, 4, 1, 256), (3, 4, 1, 64), (5, 4, 1, 128), (20, 20, 1, 64),
+                                       (40, 8, 1, 128)])
+def test_values_near_the_largest(t, T, hq, hk, d, dtype):
+    """Three keys of values 5e37, the later ones 5.4 nats above the first: no sum of weighted values may leave
+    the type's range, as none does whose weights are at most 1."""
+    n, cap = 250 - T, 250
+    q, k, v = (values(t, dtype, *s, seed=90 + i) for i, s in enumerate([(1, T, hq, d), (1, hk, cap, d), (1, hk, cap, d)]))
+    q.zero_()
+    q[..., 0] = float(d) ** 0.5
+    k.zero_()
+    k[..., 0] = -100.0
+    k[:, :, 0, 0] = 0.0
+    for at in (128, 192):
+        k[:, :, at, 0] = 5.40625
+    v.fill_(5e37)
+    out = call("tree_attention", [q, k, v, t.tensor([n], dtype=t.int32).cuda(), None], [t.empty_like(q)])[0]
+    want = np.full((1, T, hq, d), float(v[0, 0, 0, 0]))
+    # exact weights would leave v itself; what rounding does to them it does above and below the line, the
+    # 16-bit kernels' own rounding of a weight excepted
+    close(out, want, ((2 * 800 + cap) * U + POLYNOMIAL + 2 * HALF_STEP[dtype]) * want)
