@@ -6,7 +6,7 @@
 //   x y = hi hi' + hi lo' + lo hi'   (lo lo' is below 2^-22 of the product),
 // each of the three with its own accumulators for the scores, which shortens
 // the chains and adds the small terms to each other first.  Rounding to tf32 is
-// an integer addition and a mask.  Queries are split once a piece.  In plain FMA
+// an integer addition, a mask and a minimum.  Queries are split once a piece.  In plain FMA
 // 16 rows would fill the FMA pipe for longer than HBM needs.
 //
 // In P V the k index runs over the keys in the order 0 2 4 6 1 3 5 7: a thread's
@@ -44,13 +44,17 @@ __device__ __forceinline__ void pin(uint32_t& x) { asm volatile("" : "+r"(x) : :
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x) : : "memory"); }
 
 // x = hi + lo for tf32 products, which ignore the low 13 bits: hi is x rounded to
-// the 11 that count, lo the rest, of which they see 11 more.  Where x is infinite
-// hi alone carries it, and `part`, hi for the products with another value's lo
-// (which may be 0 or of the other sign), is 0.
+// the 11 that count and held at the largest finite one, lo the rest, of which they
+// see 11 more.  What is infinite or no number stands in lo alone.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = fabsf(x) == INFINITY ? 0u : __float_as_uint(x - __uint_as_float(hi));
+  const float r = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+  float h;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(h) : "f"(r), "f"(0x1.ffcp127f));
+  hi = __float_as_uint(h);
+  lo = __float_as_uint(x - h);
 }
+// `part`: hi for the products with another value's lo, 0 where x is infinite: beside
+// an infinity of one sign they could overflow to the other.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo, uint32_t& part) {
   split(x, hi, lo);
   part = fabsf(x) == INFINITY ? 0u : hi;
@@ -293,12 +297,12 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
 #pragma unroll
           for (int nb = 0; nb < DP / 8; ++nb) {
             const int ch = 2 * nb + (g >> 2);
-            uint32_t h0, l0, p0, h1, l1, p1;
-            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r, ch) + 4 * (g & 3)), h0, l0, p0);
-            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r + 1, ch) + 4 * (g & 3)), h1, l1, p1);
+            uint32_t h0, l0, h1, l1;
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r, ch) + 4 * (g & 3)), h0, l0);
+            split(*reinterpret_cast<const float*>(v_sm + at<KEYS>(r + 1, ch) + 4 * (g & 3)), h1, l1);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-              mma(o[i][nb], pl[i], p0, p1);
+              mma(o[i][nb], pl[i], h0, h1);
               mma(o[i][nb], ph[i], l0, l1);
               mma(o[i][nb], ph[i], h0, h1);
             }

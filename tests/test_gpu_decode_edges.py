@@ -126,3 +126,24 @@ def test_values_near_the_largest(t, T, hq, hk, d, dtype):
     # exact weights would leave v itself; what rounding does to them it does above and below the line, the
     # 16-bit kernels' own rounding of a weight excepted
     close(out, want, ((2 * 800 + cap) * U + POLYNOMIAL + 2 * HALF_STEP[dtype]) * want)
+
+
+@pytest.mark.parametrize("T,hq,d,cap", [(6, 2, 64, 200), (3, 8, 64, 700), (20, 2, 128, 200), (12, 12, 128, 700), (9, 3, 256, 300),
+                                        (2, 4, 64, 300), (6, 1, 256, 400)])
+def test_fp32_values_at_the_end_of_their_range(t, T, hq, d, cap):
+    """The largest finite fp32 values: in a draft that no row sees they leave no trace, in a key against a 0 of the
+    query they add 0, in values that are seen they are weighted like others."""
+    top = float(np.finfo(np.float32).max)
+    q, k, v, lengths, mask = tree_inputs(t, (T, hq, 1, d, cap, [0, 1, cap - T]), "f32", seed=95)
+    mask[:, :, 1] = False
+    mask[:, 1, 1] = False                      # nobody sees draft 1
+    for b, n in enumerate(lengths.tolist()):
+        k[b, :, n + 1], v[b, :, n + 1] = -top, -top
+        v[b, :, n, 5], v[b, :, n, 6] = -top, top * (1 - 2.0 ** -12)
+    q[..., 7] = 0.0
+    k[2, :, 0, 7] = top
+    out = call("tree_attention", [q, k, v, lengths, t.tensor(mask).cuda()], [t.full_like(q, 7.0)])[0]
+    want, size, ulps = O.tree_attention(host(q), host(k), host(v), lengths.tolist(), mask, d ** -0.5)
+    # the bound of a score counts |q| |k|, 0 at dim 7; a value cut off keeps 21 bits: 2**-21 of it
+    close(out, want, tree_tolerance(want, size, ulps, "f32") + 2.0 ** -21 * size)
+    assert status() == 0
