@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int NB = 2;
   const int lane = threadIdx.x & 31, hpw = 32 / lanes, own = lane / lanes;
-  const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+  const int item = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5));  // threads may pass 32 bits, warps do not
   const int token = item / a.chunks;
   if (token >= a.tokens) return;
   const int b = token / a.seq, t = token - b * a.seq;

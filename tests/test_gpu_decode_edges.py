@@ -6,6 +6,7 @@ test derives what it adds.
 import numpy as np
 import pytest
 
+from hackathon_b200 import rotary
 from oracle import decode as O
 from test_gpu_decode import HALF_STEP, U, call, close, host, status, tree_inputs, tree_tolerance, values
 
@@ -147,3 +148,17 @@ def test_fp32_values_at_the_end_of_their_range(t, T, hq, d, cap):
     # the bound of a score counts |q| |k|, 0 at dim 7; a value cut off keeps 21 bits: 2**-21 of it
     close(out, want, tree_tolerance(want, size, ulps, "f32") + 2.0 ** -21 * size)
     assert status() == 0
+
+
+def test_rotary_past_32_bit_thread_counts(t):
+    """More warps than 2**27: every token is turned, and once."""
+    n, d = (1 << 27) + 1000, 4
+    x = t.empty(1, n, 1, d, dtype=t.bfloat16, device="cuda").normal_(generator=t.Generator(device="cuda").manual_seed(1))
+    pos = t.arange(n, dtype=t.int32, device="cuda")
+    steps = rotary.rotary_steps(d, 10000.0)[0]
+    places = [slice(0, 1500), slice((1 << 26) - 50, (1 << 26) + 50), slice(n - 1500, n)]
+    before = [host(x[:, p]) for p in places]
+    call("rotary_embedding", [x, pos, t.tensor(steps).cuda()], [x])  # in place: a token taken twice turns twice
+    for p, a in zip(places, before):
+        want = O.turned(a, host(pos[p]).astype(np.int64)[None], steps, 1.0, 0)
+        close(x[:, p], want, 2.0 ** -20 * O.pair_size(a, d, 1.0, 0) + HALF_STEP["bf16"] * np.abs(want) + 1e-7)
