@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256, 4) tree_join_kernel(const Args a, int til
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int item = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+  const int item = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5));  // threads may pass 32 bits, warps do not
   if (item >= items) return;
   const int per = tile_rows / RW, seg = item / per, r0 = (item - seg * per) * RW;
   const int bh = seg / a.rtiles, row0 = (seg - bh * a.rtiles) * tile_rows + r0;
@@ -351,7 +351,7 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
     const int rw = p.head_dim <= 128 && pl.segments * pl.rows > 64ll * sm_count() ? 4 : 1;
     const int items = (int)(pl.segments * pl.rows / rw);
     auto join = p.head_dim > 128 ? tree_join_kernel<2, 1> : rw == 4 ? tree_join_kernel<1, 4> : tree_join_kernel<1, 1>;
-    return launch_pdl(join, (items + 7) / 8, 256, 0, s, a, pl.rows, items);
+    return launch_pdl(join, (int)((items + 7ll) / 8), 256, 0, s, a, pl.rows, items);
   }
   return launch_pdl(tree_rows_kernel, (int)rows, 128, 0, s, a);
 }

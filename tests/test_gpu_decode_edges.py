@@ -162,3 +162,21 @@ def test_rotary_past_32_bit_thread_counts(t):
     for p, a in zip(places, before):
         want = O.turned(a, host(pos[p]).astype(np.int64)[None], steps, 1.0, 0)
         close(x[:, p], want, 2.0 ** -20 * O.pair_size(a, d, 1.0, 0) + HALF_STEP["bf16"] * np.abs(want) + 1e-7)
+
+
+def test_tree_attention_past_32_bit_thread_counts(t):
+    """More query rows at one row a joining warp than 2**27 warps: the rows of segments that were cut are all joined."""
+    hk, g, d, cap = 130, (1 << 20) - 16, 136, 260
+    if t.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GB of device memory")
+    q = t.zeros(1, 1, hk * g, d, dtype=t.bfloat16, device="cuda")
+    k, v = values(t, "bf16", 1, hk, cap, d, seed=1), values(t, "bf16", 1, hk, cap, d, seed=2)
+    out = t.full_like(q, 7.0)
+    call("tree_attention", [q, k, v, t.tensor([cap - 1], dtype=t.int32).cuda(), None], [out])
+    # a query of zeros: equal weights, the mean of the values
+    want = v[0].double().mean(1)
+    size = v[0].double().abs().mean(1)
+    for h in range(hk):
+        off = (out[0, 0, h * g:(h + 1) * g].double() - want[h]).abs().amax(0)
+        assert (off <= (2.0 ** -16 + 2 * cap * U) * size[h] + HALF_STEP["bf16"] * want[h].abs() + 1e-7).all(), h
+    assert status() == 0
