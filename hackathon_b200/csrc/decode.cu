@@ -295,7 +295,8 @@ int launch_tree_attn(const c3b_tensor* in, int n_in, const c3b_tensor* out, int 
   C3B_REQUIRE(p.batch >= 0 && p.tokens >= 0 && p.heads > 0 && p.kv_heads > 0 && p.heads % p.kv_heads == 0,
               "tree attention: heads is a multiple of kv_heads");
   C3B_REQUIRE(p.head_dim >= 1 && p.head_dim <= 256, "tree attention: head_dim is 1 to 256");
-  C3B_REQUIRE(p.capacity >= 0 && p.capacity < (1ll << 31), "tree attention: bad capacity");
+  // rows are rounded up to whole units in 32 bits
+  C3B_REQUIRE(p.capacity >= 0 && p.capacity <= (1ll << 31) - 256, "tree attention: the capacity is 0 to 2^31 - 256");
   // the kernels multiply by scale / ln 2
   C3B_REQUIRE(std::isfinite(p.scale * 1.4426950408889634f) && p.scale > 0.f, "tree attention: the scale is positive and below 2e38");
   const int64_t rows = (int64_t)p.batch * p.tokens * p.heads;

@@ -355,7 +355,8 @@ typedef struct {
  * sequence sees its committed rows and the drafts j with mask[i][j] != 0 (one
  * byte each): mask_mode 0 none given, a chain (j <= i); 1 [T, T] for all
  * sequences; 2 [B, T, T].  A row that sees nothing is zero.  Head h reads kv
- * head h / (heads / kv_heads).  head_dim 1 to 256.  T = 1 is the decode step.
+ * head h / (heads / kv_heads).  head_dim is 1 to 256, capacity up to 2^31 - 256.
+ * T = 1 is the decode step.
  * Second output: a workspace of c3b_tree_attention_workspace bytes, 16-byte
  * aligned (may be left out where that is 0).  Its contents do not outlast the
  * call; calls that overlap on the GPU need one each. */
