@@ -755,7 +755,7 @@ def _b_tree_attention(ins, outs, p):
     else:
         raise ValueError(f"tree_attention: the mask is [{T}, {T}] or [{B}, {T}, {T}]")
     scale = p.get("scale")
-    tp.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    tp.scale = float(scale) if scale is not None else 1.0 / math.sqrt(max(D, 1))  # no head_dim of 0: refused at the launch
     tin = [q.t(), k.t(), v.t(), lengths.t()] + ([mask.t()] if mask is not None else [])
     touts = [_exact_out(outs, 0, q.shape, q.dtype, "the output")] + [o.t() for o in outs[1:]]
     return Prepared([Launch(L.K_TREE_ATTN, tin, touts, tp)], [q.shape] + [o.shape for o in outs[1:]])

@@ -4,7 +4,7 @@ import pytest
 
 from hackathon_b200 import _lib as L
 from hackathon_b200.kernels import Desc
-from test_decode import launch
+from test_decode import Space, launch
 
 
 @pytest.mark.parametrize("capacity", [(1 << 31) - 255, (1 << 31) - 1])
@@ -16,3 +16,10 @@ def test_tree_attention_refuses_a_capacity_whose_units_pass_32_bits(capacity):
     lengths, work = Desc(3 * gb, L.I32, (1,)), Desc(4 * gb, L.U8, (1 << 24,))
     with pytest.raises(RuntimeError, match="capacity"):
         launch("tree_attention", [q, k, v, lengths], [out, work], {})
+
+
+def test_tree_attention_refuses_heads_of_no_elements():
+    n = Space()
+    q, k, v, out = (n(L.BF16, *s) for s in ((2, 3, 4, 0), (2, 2, 16, 0), (2, 2, 16, 0), (2, 3, 4, 0)))
+    with pytest.raises(RuntimeError, match="head_dim"):
+        launch("tree_attention", [q, k, v, n(L.I32, 2)], [out], {})
