@@ -31,7 +31,8 @@ from .kernels import Desc, prepare, registered as _prepared_names, resolve as _r
 KernelFunc = Callable[..., None]
 _registry: Dict[str, KernelFunc] = {}
 
-_TYPESTR = {"<f4": L.F32, "<i8": L.I64, "<i4": L.I32, "<f2": L.F16, "|u1": L.U8, "|b1": L.U8, "<V2": L.BF16}
+_TYPESTR = {"<f4": L.F32, "<i8": L.I64, "<i4": L.I32, "<f2": L.F16, "|u1": L.U8, "<V2": L.BF16}
+_MASK = {"tree_attention": 4}  # names with an input that may be a bool array, read as bytes; kernels write no bools
 
 
 def register(name: str) -> Callable[[KernelFunc], KernelFunc]:
@@ -77,8 +78,8 @@ def _is_torch(x: Any) -> bool:
     return type(x).__module__.startswith("torch")
 
 
-def describe(x: Any) -> Desc:
-    """Device array -> Desc (pointer, dtype, shape); must be C-contiguous."""
+def describe(x: Any, mask: bool = False) -> Desc:
+    """Device array -> Desc (pointer, dtype, shape); must be C-contiguous.  Bool arrays only as a mask."""
     if _is_torch(x):
         import torch
         if not x.is_cuda:
@@ -86,7 +87,9 @@ def describe(x: Any) -> Desc:
         if not x.is_contiguous():
             raise ValueError("kernel arrays must be C-contiguous")
         dmap = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16, torch.int64: L.I64,
-                torch.int32: L.I32, torch.uint8: L.U8, torch.bool: L.U8}
+                torch.int32: L.I32, torch.uint8: L.U8}
+        if mask:
+            dmap[torch.bool] = L.U8
         if x.dtype not in dmap:
             raise TypeError(f"unsupported dtype {x.dtype}")
         return Desc(int(x.data_ptr()), dmap[x.dtype], tuple(int(d) for d in x.shape))
@@ -105,6 +108,8 @@ def describe(x: Any) -> Desc:
         if tuple(reversed(exp)) != tuple(st) and int(np.prod(shape)) > 1:
             raise ValueError("kernel arrays must be C-contiguous")
     ts = cai["typestr"]
+    if mask and ts == "|b1":
+        ts = "|u1"
     if ts not in _TYPESTR:
         raise TypeError(f"unsupported dtype {ts}")
     return Desc(int(cai["data"][0]), _TYPESTR[ts], shape)
@@ -151,7 +156,7 @@ def _make(name: str) -> KernelFunc:
             if x is None:
                 ins.append(None)
                 continue
-            d = describe(x)
+            d = describe(x, mask=i == _MASK.get(name))
             if i == 1 and name in _HOST_SECOND:
                 d.host = _host_values(x)
             ins.append(d)
@@ -207,7 +212,7 @@ for _name in _prepared_names():
 def _ready(name: str, inputs: List[Any], outputs: List[Any], params: Dict[str, Any]):
     """What launches of this signature need: kernel id, inputs, tensor records (without addresses),
     parameter block, bytes of a workspace to bring, and outputs given in another than their logical shape."""
-    ins = [None if x is None else describe(x) for x in inputs]
+    ins = [None if x is None else describe(x, mask=i == _MASK.get(name)) for i, x in enumerate(inputs)]
     outs = [describe(o) for o in outputs]
     workspace = 0
     if name == "tree_attention" and len(outs) == 1 and len(ins) > 1 and \
