@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -72,13 +73,20 @@ def torch_call_needs_build() -> bool:
 
 
 def build_torch_call(force: bool = False):
+    """The binding makes calls from torch tensors faster; without it the registry takes its general path, so a compiler
+    that fails on torch's headers is a warning."""
     if not force and not torch_call_needs_build():
         return
-    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    tmp = TORCH_LIB.with_suffix(f".{os.getpid()}.tmp")
     cmd = torch_call_command(tmp)
-    if cmd is not None:
-        subprocess.run(cmd, check=True)
+    if cmd is None:
+        return
+    done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    if done.returncode == 0:
         os.replace(tmp, TORCH_LIB)
+        return
+    tmp.unlink(missing_ok=True)
+    warnings.warn("the torch binding was not built: " + done.stdout.decode(errors="replace")[-2000:])
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
