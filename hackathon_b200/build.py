@@ -12,9 +12,11 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 import warnings
 from pathlib import Path
 
@@ -24,7 +26,6 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libc3b200.so"
 TORCH_SRC = CSRC / "torch_call.cpp"
-TORCH_LIB = PKG / "_torch_call.so"  # the fast calls from torch tensors; only where torch is installed
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -53,9 +54,23 @@ def _torch_dir():
     return Path(spec.origin).parent if spec and spec.origin else None
 
 
+def torch_version():
+    """Version of the torch that is installed, without importing it; None where there is none."""
+    torch = _torch_dir()
+    if torch is None or not (torch / "version.py").exists():
+        return None
+    found = re.search(r"^__version__ = ['\"](.+?)['\"]", (torch / "version.py").read_text(), re.M)
+    return found.group(1) if found else None
+
+
+def torch_lib(version) -> Path:
+    """The torch binding (fast calls from torch tensors) for one version of torch and this Python.  It reads tensors
+    through inlined accessors, so another version's object must not be loaded."""
+    return PKG / f"_torch_call.{sysconfig.get_config_var('SOABI')}.torch-{version}.so"
+
+
 def torch_call_command(out: Path):
     """g++ command of the torch binding, or None where torch or Python's headers are missing."""
-    import sysconfig
     torch, python = _torch_dir(), Path(sysconfig.get_paths()["include"])
     cxx = shutil.which("g++")
     if torch is None or cxx is None or not (python / "Python.h").exists() or not (torch / "lib" / "libc10_cuda.so").exists():
@@ -68,7 +83,8 @@ def torch_call_command(out: Path):
 
 
 def torch_call_needs_build() -> bool:
-    t = TORCH_LIB.stat().st_mtime if TORCH_LIB.exists() else -1.0
+    lib = torch_lib(torch_version())
+    t = lib.stat().st_mtime if lib.exists() else -1.0
     return any(p.stat().st_mtime > t for p in (TORCH_SRC, INCLUDE / "c3b200.h"))
 
 
@@ -77,13 +93,14 @@ def build_torch_call(force: bool = False):
     that fails on torch's headers is a warning."""
     if not force and not torch_call_needs_build():
         return
-    tmp = TORCH_LIB.with_suffix(f".{os.getpid()}.tmp")
+    lib = torch_lib(torch_version())
+    tmp = lib.with_suffix(f".{os.getpid()}.tmp")
     cmd = torch_call_command(tmp)
     if cmd is None:
         return
     done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if done.returncode == 0:
-        os.replace(tmp, TORCH_LIB)
+        os.replace(tmp, lib)
         return
     tmp.unlink(missing_ok=True)
     warnings.warn("the torch binding was not built: " + done.stdout.decode(errors="replace")[-2000:])

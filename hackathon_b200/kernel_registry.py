@@ -21,11 +21,14 @@ The launch stream is the caller's current stream (CuPy's or torch's), as in
 from __future__ import annotations
 
 import ctypes as C
+from importlib.machinery import ExtensionFileLoader
+from importlib.util import module_from_spec, spec_from_loader
 from typing import Any, Callable, Dict, List, Optional
 
 import numpy as np
 
 from . import _lib as L
+from .build import torch_lib
 from .kernels import Desc, prepare, registered as _prepared_names, resolve as _resolve_builder, tree_attention_workspace
 
 KernelFunc = Callable[..., None]
@@ -236,9 +239,11 @@ def _bound():
     global _torch_call
     if _torch_call is None:
         try:
-            import torch  # noqa: F401  (its libraries are the module's)
-            from . import _torch_call as m
-        except ImportError:
+            import torch  # its libraries are the module's
+            path = str(torch_lib(torch.__version__))
+            loader = ExtensionFileLoader(f"{__package__}._torch_call", path)
+            m = module_from_spec(spec_from_loader(loader.name, loader))
+        except ImportError:  # no torch, or no binding that was built for this one
             _torch_call = False
             return False
         lib = L.lib()
