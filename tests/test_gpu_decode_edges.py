@@ -180,3 +180,32 @@ def test_tree_attention_past_32_bit_thread_counts(t):
         off = (out[0, 0, h * g:(h + 1) * g].double() - want[h]).abs().amax(0)
         assert (off <= (2.0 ** -16 + 2 * cap * U) * size[h] + HALF_STEP["bf16"] * want[h].abs() + 1e-7).all(), h
     assert status() == 0
+
+
+# tokens, q heads, kv heads, capacity, lengths: 6, 12, 16 and 40 rows of a kv head, cut and uncut, ragged
+HEADS = [(2, 6, 2, 900, [898, 0, 131]), (3, 8, 2, 700, [697, 64]), (4, 4, 1, 200, [196, 3]), (10, 4, 1, 600, [590, 255, 1])]
+
+
+def exact_tolerance(want, size, ulps, dtype, n, v_max):
+    """Up to 16 rows (any number at head sizes above 128) 16-bit weights go with what their rounding leaves: off by half a
+    step of half a step, in fp16 at least by 2**-32 of the largest weight for each of n keys."""
+    weights = 0.0 if dtype == "f32" else HALF_STEP[dtype] ** 2
+    err = (2 * ulps * U + weights) * size + (n * 2.0 ** -32 * v_max if dtype == "fp16" else 0.0)
+    return (1 + HALF_STEP[dtype]) * err + HALF_STEP[dtype] * np.abs(want) + 1e-7
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("d", [256, 136, 200, 132, 128, 64, 40, 32, 8, 4])
+@pytest.mark.parametrize("case", HEADS)
+def test_head_sizes(t, case, d, dtype):
+    """Boxes wider than a head, heads of up to two 128-dim halves in the kernels and in the join, whole and in part."""
+    T, hq, hk, cap, lengths = case
+    q, k, v, n, mask = tree_inputs(t, (T, hq, hk, d, cap, lengths), dtype, seed=75)
+    out = call("tree_attention", [q, k, v, n, t.tensor(mask).cuda()], [t.full_like(q, 7.0)])[0]
+    assert status() == 0
+    want, size, ulps = O.tree_attention(host(q), host(k), host(v), lengths, mask, d ** -0.5)
+    if T * hq // hk <= 16 or d > 128:
+        tol = exact_tolerance(want, size, ulps, dtype, cap, host(v.abs().max()))
+    else:
+        tol = tree_tolerance(want, size, ulps, dtype) + POLYNOMIAL * size
+    close(out, want, tol)
