@@ -209,3 +209,20 @@ def test_head_sizes(t, case, d, dtype):
     else:
         tol = tree_tolerance(want, size, ulps, dtype) + POLYNOMIAL * size
     close(out, want, tol)
+
+
+@pytest.mark.parametrize("g", [4, 16, 40])
+def test_fp32_sums_over_many_rows_do_not_drift(t, g):
+    """Equal weights (queries of zeros) on values with a mean, 40000 rows of 160 heads, so that each block adds up
+    thousands of rows.  Roundings to nearest are as often up as down: over 10240 sums their mean is within
+    8 sigma = 8 sqrt(additions / 3) u / sqrt(10240); a value itself may lose 2**-21 of it.  Sums that are cut off at every
+    addition would all fall short, by 7e-6."""
+    hk, n, d = 160, 40_000, 64
+    k = t.zeros(1, hk, n + 1, d, device="cuda")
+    v = t.empty_like(k).normal_(1.0, 0.25, generator=t.Generator(device="cuda").manual_seed(3))
+    q = t.zeros(1, 1, hk * g, d, device="cuda")
+    out = call("tree_attention", [q, k, v, t.tensor([n], dtype=t.int32).cuda(), None], [t.empty_like(q)])[0]
+    want = t.stack([v[0, h].double().mean(0) for h in range(hk)])
+    off = (out.view(hk, g, d).double() / want[:, None] - 1).mean((0, 2)).abs().max().item()
+    assert off <= 2.0 ** -21 + 8 * (n / 8 / 3) ** 0.5 * U / (hk * d) ** 0.5
+    assert status() == 0
