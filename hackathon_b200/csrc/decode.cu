@@ -11,7 +11,10 @@ namespace dec {
 
 // Any type, head size up to 256 and alignment: one block for each query row,
 // four warps stride over the cache rows, each with its own running maximum and
-// sum, joined at the end.
+// sum, joined at the end.  It is there for what the others cannot take, not for
+// speed: each query row reads its cache for itself in 2- or 4-byte pieces.  8 x 1
+// tokens, 32 / 8 heads of 128 one element off alignment, 2000 rows: 1.76 ms in
+// bf16, where the aligned call takes 28 us; heads of 100: 1.50 ms.
 __global__ void __launch_bounds__(128) tree_rows_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int PL = 8;  // elements a lane: head_dim <= 256
@@ -187,7 +190,9 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
     unit = f32_unit(pl.dp, pl.rows);
     per_sm = 1;
   } else if (pl.dp <= 128 && rows > 32) {
-    // 33 to 128 rows: one tile for both softmax groups; more: a tile each
+    // 33 to 128 rows: one tile for both softmax groups; more: a tile each.  At head size 128 mma.sync takes 52 us for 17
+    // rows and this kernel 67, but 81 against 71 for 33 rows and 169 against 79 for 128 (16 sequences of 500 to 4000
+    // rows, 8 heads).  At head size 64 mma.sync would stay ahead up to 64 rows (48 us against 54).
     pl.kernel = TC16;
     unit = 128;
     pl.rows = rows <= 128 ? 128 : 256;
@@ -204,8 +209,10 @@ static Plan make_plan(const c3b_tree_attn_params& p, int dtype) {
   pl.split = p.capacity > 256;
   pl.min_units = 256 / unit;
   // Starting and ending a piece costs about as much as 3 units (queries, masks of the last unit, the join of the
-  // groups), 8 of the tcgen05 kernel's: 0, 2, 4 and 8 measured 39, 22, 24 and 28 us for 128 short fp32 segments and
-  // 242, 231, 223 and 212 us for 256 segments of 512 rows a kv head.
+  // groups), 8 of the tcgen05 kernel's.  0, 1, 3 and 8 of them measured 34, 28, 24 and 26 us for 128 fp32 segments of 0 to
+  // 1000 rows, 50, 44, 38 and 40 us for 512 bf16 segments of 100 to 1500, 67, 65, 65 and 65 us for 256 of 500 to 7000;
+  // tcgen05: 0, 4, 8 and 16 of them 202, 118, 106 and 110 us for 512 segments of 100 to 1500 rows (64 query rows
+  // each), 179, 169, 167 and 173 us for 128 of 2000 to 4100 (512 query rows).
   pl.ahead = pl.kernel == TC16 ? 8 : 3;
   const int64_t grid = pl.split ? pl.segments * units : pl.segments;
   if (pl.segments * (units + pl.ahead) >= (1ll << 31) || pl.segments * pl.rows >= (1ll << 31)) return Plan{};  // 32-bit counts

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
         if (lane == 0) mbar_arrive(&empty[st]);
       }
 
-      // ---- join the four key groups
+      // ---- join the key groups
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
                 *d = x;
               }
           if (round == 0 && KG == 0 && lane < S::ROWS) {
-            // the rows' maxima and sums over the four groups
+            // the rows' maxima and sums over the groups
             float mx = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int k = 0; k < NW; ++k) mx = fmaxf(mx, m_sm[k * S::ROWS + lane]);

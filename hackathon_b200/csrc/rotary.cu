@@ -285,6 +285,8 @@ __device__ __forceinline__ T* heads_of(const Args& a, int role, int token, int b
 
 // Narrower pieces than 16 bytes, or weights of each head: a warp takes one token and
 // chunk_heads of its heads; NB heads are loaded before the first is stored.
+// 16 x 512 tokens, 32 + 8 + 8 heads of 128 in bf16, norm and turn (rotary_bulk_kernel: 45 us, floor 31): weights of each
+// head 80 us, which each lane reads for each head; 8-byte pieces 61 us, 4-byte pieces 90 us.
 template <typename T, int VEC, int MODE, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const Args a, const int lanes) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -516,7 +518,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) rotary_bulk_kernel(const Args a
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
 
-// Any even rotary size, head size and alignment: a warp per head, one pair a lane.
+// Any even rotary size, head size and alignment: a warp per head, one pair a lane.  The call above, one element off
+// alignment: 221 us; 32 heads of 50, 10 turned, 16 x 512 tokens: 125 us for a floor of 8.
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_any_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -317,7 +317,10 @@ typedef struct {
 /* ---------------------------------------------------- cached decoding
  * No counterpart in the reference, whose decoder Transformers have learned
  * positions and no cache.  q, k, v and caches share one type (f32, bf16 or
- * fp16); all arithmetic is fp32, rounded once to the output's type.
+ * fp16).  Sums, norms and softmax statistics are fp32, and outputs are rounded
+ * once.  The attention also rounds its weights to 16 bits before they multiply v,
+ * where q is 16 bits and a kv head has more than 16 query rows (tokens * heads /
+ * kv_heads) of head_dim up to 128.
  *
  * Caches are [batch, kv_heads, capacity, head_dim].  lengths i32 [batch] counts
  * each sequence's committed rows; the rows of the T tokens of a call follow
