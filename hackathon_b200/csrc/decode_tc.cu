@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           top *= a.scale_log2;
           if (!(top < INFINITY)) l = NAN;  // a NaN or an infinite score: so is the row, as its definition has it
-          const bool grow = top > m + (dec::LAG + dec::lift(H16));  // m: the reference of dec::LAG and dec::lift
+          // m: the reference of dec::LAG and dec::lift; a difference of two scores is exact where their sum with LAG is not
+          const bool grow = top - m > dec::LAG + dec::lift(H16);
           if (__any_sync(0xffffffffu, grow)) {
             const float mn = grow ? top - dec::lift(H16) : m;
             const float f = mn == -INFINITY ? 1.f : exp2_sfu(m - mn);
@@ -392,6 +393,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float neg = m == -INFINITY ? 0.f : -m;
           const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), neg2 = make_float2(neg, neg);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          // One fused multiply-add from score to exponent, as long as the rounding of m is a fraction of a power of two.
+          // Scores beyond that are rounded like the maximum that m came from, then subtracted, which keeps exponents
+          // below LAG + lift.
           auto weights = [&](auto masked) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -402,8 +406,11 @@ __global__ void __launch_bounds__(THREADS, 1)
               uint32_t pk[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
-                float2 z = __ffma2_rn(make_float2(x[2 * q], x[2 * q + 1]), sc2, neg2);
-                float2 e;
+                float2 z = make_float2(x[2 * q], x[2 * q + 1]), e;
+                if constexpr (decltype(masked)::value)  // not packed, whose product and sum the compiler would fuse
+                  z = make_float2(__fadd_rn(__fmul_rn(z.x, sc2.x), neg), __fadd_rn(__fmul_rn(z.y, sc2.y), neg));
+                else
+                  z = __ffma2_rn(z, sc2, neg2);
                 if constexpr (decltype(masked)::value) {  // the SFU, whose 2^-inf is 0
                   e.x = bits >> (2 * q) & 1 ? exp2_sfu(z.x) : 0.f;
                   e.y = bits >> (2 * q + 1) & 1 ? exp2_sfu(z.y) : 0.f;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               st16(t_s + 16 * c, pk);  // columns whose scores have been read
             }
           };
-          if (open) {
+          if (open || __any_sync(0xffffffffu, fabsf(top) > 4194304.f)) {  // 2^22
             weights(std::true_type());
           } else {
             weights(std::false_type());
@@ -455,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           float x = 0.f;
           for (int c = 0; c < a.d; ++c)
             x = fmaf(load_as_f32(q, a.dtype, c), load_as_f32(kr, a.dtype, c), x);
-          const float p = exp2_sfu(fmaf(x, a.scale_log2, m == -INFINITY ? 0.f : -m));
+          const float p = exp2_sfu(__fadd_rn(__fmul_rn(x, a.scale_log2), m == -INFINITY ? 0.f : -m));
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (c0 + c < a.d) o[c] += p * load_as_f32(vr, a.dtype, c0 + c);

@@ -226,3 +226,23 @@ def test_fp32_sums_over_many_rows_do_not_drift(t, g):
     off = (out.view(hk, g, d).double() / want[:, None] - 1).mean((0, 2)).abs().max().item()
     assert off <= 2.0 ** -21 + 8 * (n / 8 / 3) ** 0.5 * U / (hk * d) ** 0.5
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("cap", [250, 700])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,hq,hk", SHAPES)
+def test_scores_too_large_for_a_fraction(t, T, hq, hk, d, cap, dtype):
+    """Equal scores of 2**33 and more, where fp32's steps are hundreds of powers of two: equal weights all the same, since
+    a score less itself is 0."""
+    n = cap - T
+    q, k, v = (values(t, dtype, *s, seed=100 + i) for i, s in enumerate([(1, T, hq, d), (1, hk, cap, d), (1, hk, cap, d)]))
+    q.fill_(1.65625 * (2.0 ** 15 if dtype == "fp16" else 2.0 ** 30))  # no power of two: products with 1 / ln 2 are rounded
+    k.fill_(1.71875 * (2.0 ** 15 if dtype == "fp16" else 2.0 ** 30))
+    out = call("tree_attention", [q, k, v, t.tensor([n], dtype=t.int32).cuda(), None], [t.empty_like(q)])[0]
+    vv = v[0, 0].double()
+    for tok in range(T):
+        rows = n + tok + 1
+        want, size = host(vv[:rows].mean(0)), host(vv[:rows].abs().mean(0))
+        half = HALF_STEP[dtype]
+        close(out[0, tok], np.broadcast_to(want, (hq, d)), (rows * U + half) * size + half * np.abs(want) + 1e-7)
