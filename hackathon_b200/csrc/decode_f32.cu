@@ -221,7 +221,7 @@ __global__ void __launch_bounds__((Shape<DP, MT, NW>::THREADS), 1)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = (acc[i][0][j] + (acc[i][1][j] + acc[i][2][j])) * a.scale_log2;
+          for (int j = 0; j < 4; ++j) s[i][j] = __fmul_rn(acc[i][0][j] + (acc[i][1][j] + acc[i][2][j]), a.scale_log2);
         // ---- mask
         const int key0 = u * KEYS + kg * 8;
         const bool open = key0 + 8 > w.n;  // the warp's keys reach past the committed rows

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
 #pragma unroll
           for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][nb][j] *= a.scale_log2;
+            for (int j = 0; j < 4; ++j) s[i][nb][j] = __fmul_rn(s[i][nb][j], a.scale_log2);  // rounded for all its uses
         if (open) {
           const int row = r0 + (lane & (S::ROWS - 1));  // whose keys the lane looks up
           const uint32_t mine = dec::see<16>(a, w, row < a.rows ? dec::token_of(a, row) : 0, row < a.rows, key0, lane);
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__((Shape<DP, MT>::THREADS), (Shape<DP, MT>::PAIR
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             top[i][half] = x;
-            grow = grow || x > m[i][half] + (dec::LAG + dec::lift(H16));
+            grow = grow || x - m[i][half] > dec::LAG + dec::lift(H16);  // the sum of the two would be rounded above 2^24
           }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll

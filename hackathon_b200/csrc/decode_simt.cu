@@ -182,7 +182,7 @@ __global__ void __launch_bounds__((Shape<DP, RW>::THREADS), 1)
               x[0] += __shfl_xor_sync(0xffffffffu, x[0], half);
             }
           }
-          s[pass] = x[0] * a.scale_log2;
+          s[pass] = __fmul_rn(x[0], a.scale_log2);
         }
         const int key0 = u * KEYS + warp * S::KPW;
         const bool open = key0 + S::KPW > w.n;  // the warp's keys reach past the committed rows

@@ -246,3 +246,21 @@ def test_scores_too_large_for_a_fraction(t, T, hq, hk, d, cap, dtype):
         want, size = host(vv[:rows].mean(0)), host(vv[:rows].abs().mean(0))
         half = HALF_STEP[dtype]
         close(out[0, tok], np.broadcast_to(want, (hq, d)), (rows * U + half) * size + half * np.abs(want) + 1e-7)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("base,step", [((4096.0, 4080.0), 7), ((8192.0, 8160.0), 8), ((2048.0, 2040.0), 10)])
+@pytest.mark.parametrize("T,hq,hk", SHAPES)
+def test_large_scores_a_step_apart(t, T, hq, hk, base, step, dtype):
+    """A score of about 2**24 to 2**27 and, units later, one a few nats above it, near where the running maximum is
+    raised: no weight leaves the type.  The values of both keys are alike, all others' weights are 0."""
+    n, cap, d = 250 - T, 250, 64
+    q, k, v = (values(t, dtype, *s, seed=110 + i) for i, s in enumerate([(1, T, hq, d), (1, hk, cap, d), (1, hk, cap, d)]))
+    q.zero_()
+    k.zero_()
+    q[..., 0], q[..., 1] = base[0], 1.0
+    for at in (0, 128, 192):
+        k[:, :, at, 0], k[:, :, at, 1] = base[1], float(step if at else 0)
+        v[:, :, at] = 3.0
+    out = call("tree_attention", [q, k, v, t.tensor([n], dtype=t.int32).cuda(), None], [t.empty_like(q)], {"scale": 1.0})[0]
+    close(out, np.full((1, T, hq, d), 3.0), (250 * U + 2 * HALF_STEP[dtype]) * 3.0)
