@@ -180,6 +180,8 @@ def test_tree_attention_past_32_bit_thread_counts(t):
         off = (out[0, 0, h * g:(h + 1) * g].double() - want[h]).abs().amax(0)
         assert (off <= (2.0 ** -16 + 2 * cap * U) * size[h] + HALF_STEP["bf16"] * want[h].abs() + 1e-7).all(), h
     assert status() == 0
+    del q, out
+    t.cuda.empty_cache()
 
 
 # tokens, q heads, kv heads, capacity, lengths: 6, 12, 16 and 40 rows of a kv head, cut and uncut, ragged
@@ -226,6 +228,8 @@ def test_fp32_sums_over_many_rows_do_not_drift(t, g):
     off = (out.view(hk, g, d).double() / want[:, None] - 1).mean((0, 2)).abs().max().item()
     assert off <= 2.0 ** -21 + 8 * (n / 8 / 3) ** 0.5 * U / (hk * d) ** 0.5
     assert status() == 0
+    del k, v, out
+    t.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
